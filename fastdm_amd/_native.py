@@ -65,6 +65,8 @@ SIGNATURES = {
     "fdm_quant_rowwise_cat2_act": (I32, [P, P, P, I32, P, I32, I64, I32, P, I32, I64, I32, I64, P]),
     "fdm_qk_norm_rope": (I32, [P, P, P, P, P, P, P, I64, I64, I64, I64, I32, I32, F32, P]),
     "fdm_qk_norm_rope_inplace": (I32, [P, P, P, P, I64, I64, I64, I64, I64, I64, I32, I32, F32, P]),
+    "fdm_add_rms_norm": (I32, [P, P, P, P, I32, P, P, P, P, I64, I64, I64, I64, I64, F32, P]),
+    "fdm_rope_positions": (I32, [P, P, P, P, P, P, I32, I64, I64, I64, I64, I32, I32, I32, I32, I64, I64, I64, I64, I64, I64, I64, I64, F32, I32, P]),
     "fdm_absdiff_sums": (I32, [P, P, P, I64, P]),
     "fdm_abi_version": (I32, []),
     "fdm_source_digest": (C.c_char_p, []),
@@ -74,7 +76,7 @@ SIGNATURES = {
     "fdm_debug_cvt_fp8": (I32, [P, P, I64, I32, P]),
 }
 
-ABI_VERSION = 20         # FDM_ABI_VERSION of include/fastdm_amd.h these SIGNATURES were written against
+ABI_VERSION = 21         # FDM_ABI_VERSION of include/fastdm_amd.h these SIGNATURES were written against
 EPI_NONE, EPI_GELU_TANH, EPI_GELU_ERF, EPI_GATE_RESIDUAL, EPI_GATE_RESIDUAL_F32 = 0, 1, 2, 3, 4
 
 
@@ -285,6 +287,52 @@ def check(rc: int, what: str):
 
 def ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def need_gpu(what, *tensors):
+    """Every tensor on one GPU, and none that autograd would expect a gradient through (the operators have no backward)."""
+    import torch
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}: fastdm_amd operators need GPU tensors (no CPU fallback)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError(f"{what}: tensors on {dev} and {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what}: forward only -- call it under torch.no_grad() or with tensors that require no gradient")
+
+
+def row_stride(t, what):
+    """Row stride of a [rows, width] matrix whose rows may be slices of wider ones (one row: any)."""
+    rows, width = t.shape
+    assert t.stride(1) == 1 or width == 1, f"{what}: rows must be dense"
+    if rows <= 1:
+        return width
+    assert t.stride(0) >= width, f"{what}: rows overlap"
+    return t.stride(0)
+
+
+class _Here:
+    """The tensors' device is the current one already: nothing to switch."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def on_device(t):
+    """Context in which a launch goes to `t`'s device (a kernel launched on another device's stream is an error)."""
+    import torch
+    return _here if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 _raw_stream = None

@@ -90,6 +90,38 @@ def rms_norm_rows(x: torch.Tensor, weight: torch.Tensor, eps: float, rope: Optio
     return out
 
 
+def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float, quant=None,
+                 residual_out: Optional[torch.Tensor] = None) -> Tuple[Optional[torch.Tensor], Optional[Quantized], Optional[torch.Tensor]]:
+    """h = x + residual (kept in bf16); y = h / rms(h) * weight, as bf16 (quant=None) or quantised per row for the next W8A8 linear -- one pass
+    where an addition, rms_norm and quantize_rows take three, and ONE rounding of y (it is not rounded to bf16 on its way to 8 bits).
+    x, residual: [rows, width] bf16, rows may be column slices of wider matrices.  Returns (bf16 y | None, Quantized | None, h | None) like ln_modulate.
+    residual_out: where h goes (may be `residual` or `x` itself: in place).  residual=None: the norm of x alone, h is None.
+    e4m3: scale = max|y| / 448; int8: asymmetric (scale, azp), as the row quantisers."""
+    N.need_gpu("add_rms_norm", x, residual, weight, residual_out)
+    assert x.ndim == 2 and x.dtype == BF16 and weight.dtype == BF16, "add_rms_norm: x [rows, width] and weight in bf16"
+    rows, width = x.shape
+    assert 0 < width <= 65536, "add_rms_norm: 1 <= width <= 65536"
+    assert quant in QUANT_MODE, "add_rms_norm: quant None, torch.float8_e4m3fn or torch.int8"
+    assert weight.is_contiguous() and weight.numel() == width, "add_rms_norm: weight [width]"
+    xs = N.row_stride(x, "add_rms_norm")
+    rs = hs = 0
+    if residual is not None:
+        assert residual.shape == x.shape and residual.dtype == BF16, "add_rms_norm: residual as x"
+        if residual_out is None:
+            residual_out = torch.empty((rows, width), device=x.device, dtype=BF16)
+        assert residual_out.shape == x.shape and residual_out.dtype == BF16, "add_rms_norm: residual_out as x"
+        rs, hs = N.row_stride(residual, "add_rms_norm"), N.row_stride(residual_out, "add_rms_norm")
+    else:
+        assert residual_out is None, "add_rms_norm: residual_out without residual"
+    qz = _alloc_q(rows, width, quant, x.device) if quant is not None else None
+    out = torch.empty((rows, width), device=x.device, dtype=BF16) if quant is None else None
+    with N.on_device(x):
+        N.check(N.lib().fdm_add_rms_norm(N.ptr(out), N.ptr(qz.q) if qz else None, N.ptr(qz.scale) if qz else None,
+                                         N.ptr(qz.azp) if qz else None, QUANT_MODE[quant], N.ptr(x), N.ptr(residual), N.ptr(weight),
+                                         N.ptr(residual_out), rows, width, xs, rs, hs, eps, N.stream(x.device.index)), "add_rms_norm")
+    return out, qz, residual_out
+
+
 def gate_residual(res: torch.Tensor, y: torch.Tensor, gate: torch.Tensor, rows_per_batch: int) -> torch.Tensor:
     """res + gate[b]*y (model/flux.py:153-154)."""
     rows, width = res.shape

@@ -50,6 +50,55 @@ def rotary_pos_embedding(query: torch.Tensor, key: torch.Tensor, head_size: int,
     return
 
 
+def rotary_positions(query: torch.Tensor, key: Optional[torch.Tensor], head_size: int, frequencies, positions: Optional[torch.Tensor] = None,
+                     is_neox: bool = False, query_out: Optional[torch.Tensor] = None,
+                     key_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Rotary embedding at given places: query [B, S, Hq * head_size] and key [B, S, Hk * head_size] (or None) turned at positions[b, s]
+    (int32 / int64, [S] or [B, S]; None: 0 .. S - 1) by `frequencies` (layer/embeddings.py RotaryFrequencies: part of the head, scalings for long
+    contexts).  Next to rotary_pos_embedding, which reads a bf16 cos | sin table of positions 0 .. S - 1: here the angle is taken in 64 bits at any
+    place and the result is rounded once.  is_neox: pairs (i, i + rotary_dim / 2) instead of (2i, 2i + 1).  Inputs may be slices of a fused
+    projection (any batch and token strides); returns (query_out, key_out), new tensors unless given -- `query` / `key` themselves for in place,
+    a cache's slice for a key that is stored there."""
+    N.need_gpu("rotary_positions", query, key, positions, query_out, key_out, frequencies.turns)
+    rot = frequencies.rotary_dim
+    assert rot <= head_size, "rotary_positions: rotary_dim is larger than the head"
+    assert query.ndim == 3, "rotary_positions: query [B, S, heads * head_size]"
+    B, S, _ = query.shape
+
+    def side(x, out, what):
+        assert x.ndim == 3 and x.dtype == BF16, f"rotary_positions: {what} [B, S, heads * head_size] in bf16"
+        width = x.shape[2]
+        assert x.shape[0] == B and x.shape[1] == S and width % head_size == 0, f"rotary_positions: {what}'s shape"
+        if out is None:
+            out = torch.empty((B, S, width), device=x.device, dtype=BF16)
+        assert out.shape == x.shape and out.dtype == BF16, f"rotary_positions: {what}_out as {what}"
+        (x_bs, x_ts, x_es), (o_bs, o_ts, o_es) = x.stride(), out.stride()
+        assert x_es == 1 and o_es == 1, f"rotary_positions: {what}'s tokens must be dense"
+        assert (S <= 1 or o_ts >= width) and (B <= 1 or o_bs >= width), f"rotary_positions: {what}_out overlaps itself"
+        assert x_bs >= 0 and x_ts >= 0, f"rotary_positions: {what}'s strides"
+        assert out.data_ptr() != x.data_ptr() or (x_bs, x_ts) == (o_bs, o_ts), f"rotary_positions: {what} in place needs the same strides"
+        return out, width // head_size, x_bs, x_ts, o_bs, o_ts
+
+    query_out, q_heads, q_bs, q_ts, qo_bs, qo_ts = side(query, query_out, "query")
+    k_heads = k_bs = k_ts = ko_bs = ko_ts = 0
+    if key is not None:
+        key_out, k_heads, k_bs, k_ts, ko_bs, ko_ts = side(key, key_out, "key")
+    else:
+        assert key_out is None, "rotary_positions: key_out without key"
+    p_bs = p_ts = p_bytes = 0
+    if positions is not None:
+        assert positions.dtype in (torch.int32, torch.int64), "rotary_positions: positions int32 or int64"
+        assert positions.shape == (S,) or positions.shape == (B, S), "rotary_positions: positions [S] or [B, S]"
+        p_bytes, p_ts = positions.element_size(), positions.stride(-1)
+        p_bs = positions.stride(0) if positions.ndim == 2 else 0
+    with N.on_device(query):
+        N.check(N.lib().fdm_rope_positions(N.ptr(query_out), N.ptr(key_out), N.ptr(query), N.ptr(key), frequencies.turns.data_ptr(),
+                                           N.ptr(positions), p_bytes, p_bs, p_ts, B, S, q_heads, k_heads, head_size, rot, q_bs, q_ts, k_bs, k_ts,
+                                           qo_bs, qo_ts, ko_bs, ko_ts, frequencies.amplitude, int(bool(is_neox)), N.stream(query.device.index)),
+                "rotary_positions")
+    return query_out, key_out
+
+
 def gelu_and_mul(input: torch.Tensor) -> torch.Tensor:
     """operators_set.py:54-67: x[..., :d] * gelu_erf(x[..., d:]) (the gate is the SECOND half)."""
     _need_gpu(input)

@@ -5,7 +5,7 @@ These are M = batch sized (a few KFLOP) or pure table construction: the tables a
 ops exactly as the reference does (fp64 frequencies for RoPE) and cached per (ids) on the device.
 """
 import math
-from typing import List
+from typing import List, Optional, Sequence
 
 import torch
 import torch.nn.functional as F
@@ -98,6 +98,65 @@ class CombinedTimestepTextProjEmbeddings:
     def forward(self, timestep, pooled_projection):
         timesteps_emb = self.timestep_embedder.forward(self.time_proj.forward(timestep).to(dtype=pooled_projection.dtype))
         return timesteps_emb + self.text_embedder.forward(pooled_projection)
+
+
+class RotaryFrequencies:
+    """The frequencies rotary_positions (kernel/operators_set.py) turns by, made once of a model's rotary settings: pair i of `rotary_dim` / 2
+    turns by theta_i = base^(-2 i / rotary_dim) radians per position, changed for contexts longer than the trained one (`original_length`) by
+
+      "linear"      theta_i / factor: positions interpolated (Chen et al. 2023);
+      "ntk"         base * factor^(d / (d - 2)), d = rotary_dim: the slowest pair slows down by `factor`, the fastest stays;
+      "yarn"        pairs that turn more than beta_fast times within original_length stay, those under beta_slow turns slow down by `factor`, a linear
+                    ramp over the pair's index between (Peng et al. 2023; the ramp's ends at whole indices, as trained models have them);
+                    sine and cosine times attention_factor (default 0.1 ln(factor) + 1);
+      "wavelength"  pairs of wavelengths up to original_length / high_factor stay, from original_length / low_factor on they slow down by `factor`,
+                    blended by original_length / wavelength between.
+
+    Everything is computed in 64 bits; `turns` (fp64 [rotary_dim / 2], on the device) holds theta_i / (2 pi), `amplitude` what sine and cosine
+    are scaled by.  frequencies: a list of theta_i of the caller's own instead."""
+
+    def __init__(self, rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0, original_length: int = 0,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, low_factor: float = 1.0, high_factor: float = 4.0,
+                 attention_factor: Optional[float] = None, frequencies: Optional[Sequence[float]] = None, device=None):
+        if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > 256:
+            raise ValueError("RotaryFrequencies: rotary_dim is even, 2 to 256")
+        if scaling not in (None, "linear", "ntk", "yarn", "wavelength"):
+            raise ValueError(f"RotaryFrequencies: unknown scaling {scaling!r}")
+        if frequencies is not None and (scaling is not None or len(frequencies) != rotary_dim // 2):
+            raise ValueError("RotaryFrequencies: own frequencies are rotary_dim / 2 values and take no scaling")
+        if not (base > 1.0 and factor > 0.0):
+            raise ValueError("RotaryFrequencies: base > 1 and factor > 0")
+        d = rotary_dim
+        amplitude = 1.0
+        if scaling == "ntk":
+            if d < 4:
+                raise ValueError("RotaryFrequencies: ntk scaling needs rotary_dim >= 4")
+            base = base * factor ** (d / (d - 2))
+        theta = [base ** (-2.0 * i / d) for i in range(d // 2)] if frequencies is None else [float(f) for f in frequencies]
+        if scaling == "linear":
+            theta = [f / factor for f in theta]
+        elif scaling in ("yarn", "wavelength"):
+            if original_length < 1:
+                raise ValueError(f"RotaryFrequencies: {scaling} scaling needs original_length")
+            if scaling == "yarn":
+                if not beta_fast > beta_slow > 0.0:
+                    raise ValueError("RotaryFrequencies: beta_fast > beta_slow > 0")
+
+                def index(turns):       # of the pair that turns so often within original_length
+                    return d * math.log(original_length / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
+
+                first, last = max(math.floor(index(beta_fast)), 0), min(math.ceil(index(beta_slow)), d - 1)
+                slowed = [min(max((i - first) / max(last - first, 0.001), 0.0), 1.0) for i in range(d // 2)]
+                amplitude = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+            else:
+                if not high_factor > low_factor > 0.0:
+                    raise ValueError("RotaryFrequencies: high_factor > low_factor > 0")
+                slowed = [1.0 - min(max((original_length * f / (2.0 * math.pi) - low_factor) / (high_factor - low_factor), 0.0), 1.0) for f in theta]
+            theta = [f * (1.0 - s) + f / factor * s for f, s in zip(theta, slowed)]
+        if attention_factor is not None:
+            amplitude = float(attention_factor)
+        self.rotary_dim, self.amplitude, self.theta = d, amplitude, theta
+        self.turns = torch.tensor([f / (2.0 * math.pi) for f in theta], dtype=torch.float64, device=device)
 
 
 def get_1d_rotary_pos_embed(dim: int, pos: torch.Tensor, theta: float = 10000.0, freqs_dtype=torch.float64):

@@ -44,7 +44,7 @@ const char* fdm_last_hip_error_string(void);
 
 /* Bumped whenever an entry point changes its argument list: a binding built against another revision of this header must
  * refuse to run instead of passing arguments at the wrong positions. */
-#define FDM_ABI_VERSION 20
+#define FDM_ABI_VERSION 21
 int fdm_abi_version(void);
 
 /* Provenance the binary carries itself (no stamp file beside it): the content digest (64 hex digits) of every source the
@@ -437,6 +437,33 @@ int fdm_qk_norm_rope_inplace(void* qkv, const void* wq, const void* wk, const vo
                              int64_t rows, int64_t rows_per_batch, int64_t batch_row_stride,
                              int64_t row_stride, int64_t k_offset, int64_t pos_offset,
                              int heads, int head_dim, float eps, fdm_stream_t stream);
+
+/* ================= a decoder layer's rows (next to rms_norm and rotary_pos_embedding; no reference export) ================= */
+
+/* Residual addition, RMS norm and (optionally) the next W8A8 linear's per-row quantisation in one pass (ABI 21):
+ *   h = bf16(x + res), written to h_out (res and h_out both NULL: h = x, nothing is written);
+ *   y = h * weight * rsqrt(mean(h^2) + eps)         fp32, one rounding:
+ *   quant_mode 0: out_bf16 = bf16(y);  1: out_scale = max(max|y|, 1e-12) / 448, out_q = e4m3(y / out_scale);
+ *   quant_mode 2: out_scale = (max y - min y) / 255, out_azp = -128 - rint(min y / out_scale), out_q = rint(y / out_scale) + out_azp (the spread
+ *   counts as at least max|y| / 16 and 1e-12: a row of one value stays representable).
+ * x, res, h_out: [rows, width] bf16 with their own row strides (elements); outputs compact.  h_out may be x or res.  Any width <= 65536 and any
+ * (element) alignment; multiples of 8 on 16-byte aligned rows take whole vectors.  A row with a NaN or an infinity gives NaNs (its 8-bit rows: a NaN
+ * scale).  rows <= 2^31 - 1.                                                                                                          */
+int fdm_add_rms_norm(void* out_bf16, void* out_q, float* out_scale, int32_t* out_azp, int quant_mode, const void* x, const void* res,
+                     const void* weight, void* h_out, int64_t rows, int64_t width, int64_t x_row_stride, int64_t res_row_stride,
+                     int64_t h_row_stride, float eps, fdm_stream_t stream);
+
+/* Rotary positions at given places (ABI 21): q [batch, seq, q_heads * head_size] and k [batch, seq, k_heads * head_size] bf16 with batch and token
+ * strides in elements, to q_out / k_out (their own strides; q_out == q and k_out == k with equal strides: in place).  Pair i of a head's first
+ * rot_dim elements -- (2i, 2i + 1), or (i, i + rot_dim / 2) where is_neox -- turns by 2 pi * place * turns[i] and is scaled by amplitude; the rest of
+ * the head is copied.  turns: fp64 [rot_dim / 2], turns per position; the angle's fraction of a turn is taken in 64 bits, sine and cosine in fp32.
+ * positions: int32 / int64 (position_bytes 4 / 8) at positions[b * pos_batch_stride + s * pos_tok_stride], or NULL for 0 .. seq - 1.
+ * rot_dim even, <= 256.  k_heads == 0: q alone.                                                                                        */
+int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, const void* turns, const void* positions, int position_bytes,
+                       int64_t pos_batch_stride, int64_t pos_tok_stride, int64_t batch, int64_t seq, int q_heads, int k_heads, int head_size,
+                       int rot_dim, int64_t q_batch_stride, int64_t q_tok_stride, int64_t k_batch_stride, int64_t k_tok_stride,
+                       int64_t qo_batch_stride, int64_t qo_tok_stride, int64_t ko_batch_stride, int64_t ko_tok_stride, float amplitude,
+                       int is_neox, fdm_stream_t stream);
 
 /* TeaCache metric (caching/xcaching.py:214): out[0] = sum|a-b|, out[1] = sum|b| (fp32 atomics;
  * caller zeroes out[0..1]).                                                                      */
