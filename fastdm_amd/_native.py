@@ -67,6 +67,8 @@ SIGNATURES = {
     "fdm_qk_norm_rope_inplace": (I32, [P, P, P, P, I64, I64, I64, I64, I64, I64, I32, I32, F32, P]),
     "fdm_add_rms_norm": (I32, [P, P, P, P, I32, P, P, P, P, I64, I64, I64, I64, I64, F32, P]),
     "fdm_rope_positions": (I32, [P, P, P, P, P, P, I32, I64, I64, I64, I64, I32, I32, I32, I32, I64, I64, I64, I64, I64, I64, I64, I64, F32, I32, P]),
+    "fdm_attn_window_workspace_bytes": (I64, [I64, I64, I64, I32, I32, I32, I64, I64]),
+    "fdm_attn_window": (I32, [P, P, P, P, P, P, I64, I64, I64, I32, I32, I32, I64, I64, I64, I64, I64, I64, I64, I64, F32, I64, I64, P, I64, P]),
     "fdm_absdiff_sums": (I32, [P, P, P, I64, P]),
     "fdm_abi_version": (I32, []),
     "fdm_source_digest": (C.c_char_p, []),

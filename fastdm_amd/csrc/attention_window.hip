@@ -1,0 +1,520 @@
+// Causal attention with a sliding window and sinks for gfx950 (bf16, head_dim 64 or 128): prompts, chunks behind a cache, single tokens.
+//
+//   visible   the query at place p of its sequence sees key j iff  j <= p  and  (p - j < window  or  j < sinks).  The queries of a sequence are its
+//             last q_len tokens: row t is at place kv_len - q_len + t.  Rows at or past q_len, and rows that see nothing, are zeros.
+//   rows      the q heads that share a kv head are packed with the tokens: row r of (batch, kv head) is token r / G, head r % G, G = q_heads / kv_heads --
+//             one K / V tile in LDS serves all G heads, a 32-row wave spans 32 / G tokens (less of a tile lies behind the mask), and a single
+//             token's G rows are one wave's rows.
+//   tiles     a block walks the key tiles its rows see, the sinks' tiles first and then the window's; tiles in between are neither read nor
+//             multiplied.  A wave skips tiles none of its rows sees and masks element by element only where some row does not see some key.
+//   QK^T      swapped: S^T[key][q] = K . Q^T on v_mfma_f32_32x32x16_bf16: lane (q = lane & 31, h = lane >> 5) holds 16 of each 32 keys of ITS row.
+//   PV        O^T[d][q] += V^T[d][key] . P^T[key][q]: the S^T accumulator, converted pairwise to bf16, is the B operand as it is; V^T comes from the
+//             row-major tile through ds_read_b64_tr_b16.  P is rounded to bf16 (2^-9 of each weight, averaged over the keys; the row sums are those of
+//             the unrounded weights in fp32): the matrix core's operand type.
+//   softmax   one pass, running maximum and sum in fp32, exp2 domain, O and l rescaled only where a row's maximum grew by more than 2^8.
+//   waves     WR waves over rows (32 each) times WK waves over the keys of a tile: prompts WK = 1; few rows (single tokens) WR = 1, WK = 4, merged
+//             through LDS at the end.  Where the blocks would not fill the chip, a block's tile list is cut into parts that run side by side and
+//             are merged by a second small launch.
+//   NaN       what a row does not see does not reach it: masked scores are replaced, keys past kv_len are never read, and where a masked tile holds a
+//             value that is not finite (0 * NaN is NaN in the matrix core) the product is taken token by token with the invisible values zeroed.
+#include "common.h"
+#include "attn_common.h"
+
+namespace fdm {
+
+struct WindowParams {
+  bf16_t* o;
+  const bf16_t* q;
+  const bf16_t* k;
+  const bf16_t* v;
+  const int* q_lens;    // nullptr: sq
+  const int* kv_lens;   // nullptr: sk
+  int64_t q_bs, q_ts, k_bs, k_ts, v_bs, v_ts, o_bs, o_ts;
+  int batch, sq, sk, kv_heads, group;
+  int window, sinks;
+  int n_blocks;         // row blocks of a (batch, kv head)
+  int parts;            // parts a block's tile list is cut into
+  int n_items, chunk;   // batch * kv_heads * n_blocks * parts; consecutive ones per XCD
+  float scale_log2e;
+  float* ws_o;          // parts > 1: [batch * kv_heads * n_blocks][parts][rows of a block][D], unnormalised
+  float* ws_ml;         // ... [..][..][rows][2]: maximum (exp2 domain), sum
+};
+
+template <int D, int WR, int WK, int KW>
+__global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_kernel(const WindowParams p) {
+  constexpr int NT = 64 * WR * WK, RB = 32 * WR, KT = KW * WK;
+  constexpr int NKT = KW / 32;            // 32-key S^T tiles per wave and key tile
+  constexpr int CPR = D / 8;              // 16-byte pieces per key
+  constexpr uint32_t ROWB = D * 2;
+  constexpr int TILE_BYTES = KT * D * 2;
+  constexpr int LD = KT * CPR / NT;       // LDS-DMA pieces per thread and tile of K (and of V)
+  constexpr int KSTEPS = D / 16, DT = D / 32;
+  static_assert(KT * CPR % NT == 0 && LD >= 1);
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * TILE_BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave % WR, wk = wave / WR;
+  const int lq = lane & 31, h = lane >> 5;
+
+  // consecutive items run on one XCD, whose L2 then holds the window they share
+  const int xcd = blockIdx.x & 7, seat = blockIdx.x >> 3;
+  const int item = ((seat / p.chunk) * 8 + xcd) * p.chunk + seat % p.chunk;
+  if (item >= p.n_items) return;
+  const int part = item % p.parts;
+  const int unit = item / p.parts;
+  const int rb = p.n_blocks - 1 - unit % p.n_blocks;      // long lists first
+  const int bk = unit / p.n_blocks;
+  const int b = bk / p.kv_heads, kvh = bk % p.kv_heads;
+  const int G = p.group;
+
+  int q_len = p.sq, kv_len = p.sk;
+  if (p.q_lens != nullptr) q_len = min(max(p.q_lens[b], 0), p.sq);
+  if (p.kv_lens != nullptr) kv_len = min(max(p.kv_lens[b], 0), p.sk);
+  q_len = __builtin_amdgcn_readfirstlane(q_len);
+  kv_len = __builtin_amdgcn_readfirstlane(kv_len);
+  const int first = kv_len - q_len;       // place of token 0
+
+  // ---- this lane's row, and the places of the wave's and the block's rows
+  const int n_rows = p.sq * G;
+  const int row = rb * RB + wr * 32 + lq;
+  const int rowc = min(row, n_rows - 1);
+  const int tok = rowc / G, head = kvh * G + rowc % G;
+  const bool live = row < n_rows && tok < q_len;
+  const int wt_lo = (rb * RB + wr * 32) / G, wt_hi = min(min(rb * RB + wr * 32 + 31, n_rows - 1) / G, q_len - 1);
+  const int bt_lo = rb * RB / G, bt_hi = min(min(rb * RB + RB - 1, n_rows - 1) / G, q_len - 1);
+  const int wp_lo = first + wt_lo, wp_hi = first + wt_hi;        // wt_lo > wt_hi: the wave has no row
+  const int place = first + tok;
+
+  // ---- the tiles the block's rows see: [0, n_sink) and [w_begin, w_end)
+  int n_sink = 0, w_begin = 0, w_end = 0;
+  if (bt_lo <= bt_hi && first + bt_hi >= 0) {
+    const int near = max(0, first + bt_lo - p.window + 1);        // the window's first key
+    const int far = min(p.sinks, near);                           // sinks in front of it
+    n_sink = (far + KT - 1) / KT;
+    w_begin = max(near / KT, n_sink);
+    w_end = (first + bt_hi) / KT + 1;
+    w_begin = min(w_begin, w_end);
+  }
+  const int n_list = n_sink + w_end - w_begin;
+  const int i_begin = (int)((int64_t)part * n_list / p.parts), i_end = (int)((int64_t)(part + 1) * n_list / p.parts);
+  auto tile_at = [&](int i) { return i < n_sink ? i : i - n_sink + w_begin; };
+
+  const bf16_t* kbase = p.k + (int64_t)b * p.k_bs + (int64_t)kvh * D;
+  const bf16_t* vbase = p.v + (int64_t)b * p.v_bs + (int64_t)kvh * D;
+
+  // ---- Q fragments: B operand, lane holds Q[row][16 ks + 8 h .. + 8]
+  i32x4 qf[KSTEPS];
+  {
+    const bf16_t* qp = p.q + (int64_t)b * p.q_bs + (int64_t)tok * p.q_ts + (int64_t)head * D + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks) qf[ks] = *reinterpret_cast<const i32x4*>(qp + 16 * ks);
+  }
+
+  // ---- K / V staging by LDS-DMA: lane-linear destination, the swizzle is applied to the source
+  int srow[LD];
+  int kch[LD], vch[LD];
+#pragma unroll
+  for (int i = 0; i < LD; ++i) {
+    const int slot = tid + i * NT;
+    srow[i] = slot / CPR;
+    kch[i] = Swz<D>::k(srow[i], slot % CPR) * 8;
+    vch[i] = Swz<D>::v(srow[i], slot % CPR) * 8;
+  }
+  auto stage = [&](int t, int buf) {
+    uint8_t* sk_ = smem + buf * 2 * TILE_BYTES + wave * 1024;
+    uint8_t* sv_ = sk_ + TILE_BYTES;
+    const int last = kv_len - 1 - t * KT;       // >= 0: a listed tile holds a visible key
+    const bf16_t* kt_ = kbase + (int64_t)t * KT * p.k_ts;
+    const bf16_t* vt_ = vbase + (int64_t)t * KT * p.v_ts;
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const int r = min(srow[i], last);         // past the sequence: its last key again (masked)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kt_ + (int64_t)r * p.k_ts + kch[i]),
+                                       (__attribute__((address_space(3))) void*)(sk_ + i * (NT * 16)), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vt_ + (int64_t)r * p.v_ts + vch[i]),
+                                       (__attribute__((address_space(3))) void*)(sv_ + i * (NT * 16)), 16, 0, 0);
+    }
+  };
+
+  f32x16 oacc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) oacc[d][e] = 0.f;
+  float m_run = -3.0e38f, l_run = 0.f;
+  constexpr float RESCALE = 8.0f;
+
+  const int gi = lane >> 4, li = lane & 15, tq = li >> 2, tp = li & 3;
+  const uint32_t kld0 = (wk * KW + lq) * ROWB + (uint32_t)Swz<D>::k(lq, h) * 16;
+  uint32_t vld[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+    vld[d] = TILE_BYTES + (wk * KW + 4 * h + tq) * ROWB + (uint32_t)Swz<D>::v(4 * h + tq, d * 4 + 2 * (gi & 1) + (tp >> 1)) * 16 + 8 * (tp & 1);
+
+  // one key tile for this wave; base: place of its first key.  MASK: some row of the wave does not see some key
+  auto process = [&](auto mask_c, int base, uint32_t buf) {
+    constexpr bool MASK = decltype(mask_c)::value;
+    const uint8_t* sb = smem + buf;
+    f32x16 s[NKT];
+#pragma unroll
+    for (int n = 0; n < NKT; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[n][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+      for (int n = 0; n < NKT; ++n) {
+        const i32x4 kf = *reinterpret_cast<const i32x4*>(sb + (kld0 ^ (uint32_t)(ks << 5)) + n * 32 * ROWB);
+        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[ks]), s[n], 0, 0, 0);
+      }
+    if constexpr (MASK) {
+      const int at = base + 4 * h;              // element e of tile n is key at + 32 n + (e & 3) + 8 (e >> 2)
+      const int hi = place - at, lo = place - p.window - at, sink = p.sinks - at;
+#pragma unroll
+      for (int n = 0; n < NKT; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int kk = n * 32 + (e & 3) + 8 * (e >> 2);
+          if (!(kk <= hi && (kk > lo || kk < sink))) s[n][e] = -INFINITY;
+        }
+    }
+    // row maximum: med3(a, b, +inf) is max without the canonicalisation hipcc puts in front of fmaxf
+    float mx = s[0][0];
+#pragma unroll
+    for (int n = 0; n < NKT; ++n)
+#pragma unroll
+      for (int e = (n == 0 ? 1 : 0); e < 16; ++e) mx = __builtin_amdgcn_fmed3f(mx, s[n][e], __builtin_inff());
+    const float mt = cross_half_max(mx) * p.scale_log2e;
+    if (__any(mt > m_run + RESCALE)) {
+      const float m_new = fmaxf(m_run, mt);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[d][e] *= alpha;
+    }
+    float sum = 0.f;
+    i32x4 pf[NKT][2];
+#pragma unroll
+    for (int n = 0; n < NKT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][e], p.scale_log2e, -m_run));
+        s[n][e] = w;
+        sum += w;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) pf[n][u][w] = (int)pack2bf(s[n][8 * u + 2 * w], s[n][8 * u + 2 * w + 1]);
+    }
+    l_run += sum;
+    auto vfrag = [&](int n, int u, int d) {
+      const uint8_t* a = sb + vld[d] + (n * 32 + 16 * u) * ROWB;      // keys 4 h + tq, and 8 further
+      return tr_pair(a, a + 8 * ROWB);
+    };
+    if constexpr (MASK) {
+      // a masked weight is 0, and 0 * NaN is NaN: look for values that are not finite (exponent all ones)
+      u16x2 top = {0, 0};
+#pragma unroll
+      for (int n = 0; n < NKT; ++n)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const i32x4 f = vfrag(n, u, d);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, f[w] & 0x7fff7fff));
+          }
+      if (__any(top[0] >= 0x7f80 || top[1] >= 0x7f80)) {
+        for (int t = wt_lo; t <= wt_hi; ++t) {       // token by token, what it does not see zeroed
+          const int at = base + 4 * h;
+          const int hi = first + t - at, lo = hi - p.window, sink = p.sinks - at;
+          const bool mine = tok == t;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            f32x16 add = oacc[d];       // the same sums in the same order as below: the same bits
+#pragma unroll
+            for (int n = 0; n < NKT; ++n)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                i32x4 f = vfrag(n, u, d);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                  const int k0 = n * 32 + 16 * u + 8 * (w >> 1) + 2 * (w & 1);
+                  const bool see0 = k0 <= hi && (k0 > lo || k0 < sink), see1 = k0 + 1 <= hi && (k0 + 1 > lo || k0 + 1 < sink);
+                  f[w] &= (see0 ? 0x0000ffff : 0) | (see1 ? (int)0xffff0000 : 0);
+                }
+                add = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, pf[n][u]), add, 0, 0, 0);
+              }
+            if (mine) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) oacc[d][e] = add[e];
+            }
+          }
+        }
+        return;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NKT; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vfrag(n, u, d)), __builtin_bit_cast(bf16x8, pf[n][u]), oacc[d], 0, 0, 0);
+  };
+
+  if (i_begin < i_end) stage(tile_at(i_begin), 0);
+  uint32_t buf = 0;
+  for (int i = i_begin; i < i_end; ++i) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // this wave's pieces of tile i have landed ...
+    __syncthreads();                                    // ... and everybody's; the other buffer has been read
+    if (i + 1 < i_end) stage(tile_at(i + 1), buf ^ 1);
+    const int base = tile_at(i) * KT + wk * KW;
+    const bool none = wt_lo > wt_hi || base > wp_hi || (base + KW <= wp_lo - p.window + 1 && base >= p.sinks);
+    if (!none) {
+      const bool all = base + KW - 1 <= wp_lo && (base > wp_hi - p.window || base + KW <= p.sinks);
+      if (all) process(std::false_type{}, base, buf * 2 * TILE_BYTES);
+      else process(std::true_type{}, base, buf * 2 * TILE_BYTES);
+    }
+    buf ^= 1;
+  }
+
+  float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+  const int64_t unit_part = (int64_t)unit * p.parts + part;
+  if constexpr (WK == 1) {
+    if (p.parts > 1) {
+      float* wo = p.ws_o + (unit_part * RB + wr * 32 + lq) * D + 4 * h;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4)
+          *reinterpret_cast<f32x4*>(wo + 32 * d + 8 * g4) = f32x4{oacc[d][4 * g4], oacc[d][4 * g4 + 1], oacc[d][4 * g4 + 2], oacc[d][4 * g4 + 3]};
+      if (h == 0) {
+        float* ml = p.ws_ml + (unit_part * RB + wr * 32 + lq) * 2;
+        ml[0] = m_run;
+        ml[1] = l_tot;
+      }
+      return;
+    }
+    const float inv = live && l_tot != 0.f ? 1.0f / l_tot : 0.f;
+    if (row < n_rows) {
+      bf16_t* op = p.o + (int64_t)b * p.o_bs + (int64_t)tok * p.o_ts + (int64_t)head * D + 4 * h;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+          i32x2 w = {0, 0};
+          if (inv != 0.f) {
+            w[0] = (int)pack2bf(oacc[d][4 * g4] * inv, oacc[d][4 * g4 + 1] * inv);
+            w[1] = (int)pack2bf(oacc[d][4 * g4 + 2] * inv, oacc[d][4 * g4 + 3] * inv);
+          }
+          *reinterpret_cast<i32x2*>(op + 32 * d + 8 * g4) = w;
+        }
+    }
+  } else {
+    // ---- the waves' shares of the keys are merged through LDS: [wave][row][D + 4], the padding keeps rows off each other's banks
+    static_assert(WR == 1);
+    constexpr int LROW = D + 4;
+    static_assert(WK * 32 * (LROW + 2) * 4 <= 4 * TILE_BYTES);
+    float* lo = reinterpret_cast<float*>(smem);
+    float* lml = lo + WK * 32 * LROW;
+    __syncthreads();                                    // the last tile has been read
+    float* mine = lo + (wk * 32 + lq) * LROW + 4 * h;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        *reinterpret_cast<f32x4*>(mine + 32 * d + 8 * g4) = f32x4{oacc[d][4 * g4], oacc[d][4 * g4 + 1], oacc[d][4 * g4 + 2], oacc[d][4 * g4 + 3]};
+    if (h == 0) {
+      lml[(wk * 32 + lq) * 2] = m_run;
+      lml[(wk * 32 + lq) * 2 + 1] = l_tot;
+    }
+    __syncthreads();
+    constexpr int TPR = NT / 32, PER = D / TPR;         // threads per row, values each
+    static_assert(PER % 4 == 0);
+    const int r = tid / TPR, d0 = (tid % TPR) * PER;
+    float m = -3.0e38f, l = 0.f, f[WK];
+#pragma unroll
+    for (int w = 0; w < WK; ++w) m = fmaxf(m, lml[(w * 32 + r) * 2]);
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      f[w] = __builtin_amdgcn_exp2f(lml[(w * 32 + r) * 2] - m);
+      l += f[w] * lml[(w * 32 + r) * 2 + 1];
+    }
+    float acc[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) acc[j] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w)
+#pragma unroll
+      for (int j = 0; j < PER; j += 4) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(lo + (w * 32 + r) * LROW + d0 + j);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[j + c] += f[w] * x[c];
+      }
+    const int grow = rb * RB + r;
+    if (grow >= n_rows) return;
+    if (p.parts > 1) {
+      float* wo = p.ws_o + (unit_part * RB + r) * D + d0;
+#pragma unroll
+      for (int j = 0; j < PER; j += 4) *reinterpret_cast<f32x4*>(wo + j) = f32x4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]};
+      if (d0 == 0) {
+        p.ws_ml[(unit_part * RB + r) * 2] = m;
+        p.ws_ml[(unit_part * RB + r) * 2 + 1] = l;
+      }
+      return;
+    }
+    const int t = grow / G;
+    const bool ok = t < q_len && l != 0.f;
+    const float inv = ok ? 1.0f / l : 0.f;
+    bf16_t* op = p.o + (int64_t)b * p.o_bs + (int64_t)t * p.o_ts + (int64_t)(kvh * G + grow % G) * D + d0;
+#pragma unroll
+    for (int j = 0; j < PER; j += 4) {
+      i32x2 w = {0, 0};
+      if (ok) w = i32x2{(int)pack2bf(acc[j] * inv, acc[j + 1] * inv), (int)pack2bf(acc[j + 2] * inv, acc[j + 3] * inv)};
+      *reinterpret_cast<i32x2*>(op + j) = w;
+    }
+  }
+}
+
+// ---- merge of the parts: one row per D / 4 threads, o = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i in the parts' order
+template <int D>
+__global__ void __launch_bounds__(256) attn_window_merge_kernel(const WindowParams p, int rb_rows) {
+  constexpr int TPR = D / 4;
+  const int64_t n_rows = (int64_t)p.sq * p.group;
+  const int64_t idx = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (idx >= n_rows * p.batch * p.kv_heads) return;
+  const int64_t bk = idx / n_rows, row = idx % n_rows;
+  const int rb = (int)(row / rb_rows), r = (int)(row % rb_rows);
+  const int64_t unit = bk * p.n_blocks + (p.n_blocks - 1 - rb);
+  const int d0 = (threadIdx.x % TPR) * 4;
+  const int b = (int)(bk / p.kv_heads), kvh = (int)(bk % p.kv_heads);
+  const int tok = (int)(row / p.group), head = kvh * p.group + (int)(row % p.group);
+  int q_len = p.sq;
+  if (p.q_lens != nullptr) q_len = min(max(p.q_lens[b], 0), p.sq);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float m = -3.0e38f, l = 0.f;
+  for (int i = 0; i < p.parts; ++i) m = fmaxf(m, p.ws_ml[((unit * p.parts + i) * rb_rows + r) * 2]);
+  for (int i = 0; i < p.parts; ++i) {
+    const int64_t at = (unit * p.parts + i) * rb_rows + r;
+    const float f = __builtin_amdgcn_exp2f(p.ws_ml[at * 2] - m);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p.ws_o + at * D + d0);
+    l += f * p.ws_ml[at * 2 + 1];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] += f * x[c];
+  }
+  i32x2 w = {0, 0};
+  if (tok < q_len && l != 0.f) {
+    const float inv = 1.0f / l;
+    w = i32x2{(int)pack2bf(acc[0] * inv, acc[1] * inv), (int)pack2bf(acc[2] * inv, acc[3] * inv)};
+  }
+  *reinterpret_cast<i32x2*>(p.o + (int64_t)b * p.o_bs + (int64_t)tok * p.o_ts + (int64_t)head * D + d0) = w;
+}
+
+// ---- host side: which form, and into how many parts
+struct WindowPlan {
+  bool few;             // single tokens and the like: WR = 1
+  int rb_rows, kt;
+  int64_t n_blocks, units;
+  int parts;
+};
+static WindowPlan window_plan(int64_t batch, int64_t sq, int64_t sk, int64_t kv_heads, int64_t group, int head_dim, int64_t window, int64_t sinks) {
+  WindowPlan w{};
+  w.few = sq * group <= 32;
+  w.rb_rows = w.few ? 32 : 128;
+  w.kt = w.few ? (head_dim == 128 ? 128 : 256) : 64;
+  w.n_blocks = (sq * group + w.rb_rows - 1) / w.rb_rows;
+  w.units = batch * kv_heads * w.n_blocks;
+  // tiles a block walks at most, whatever the lengths on the device say
+  const int64_t span = w.rb_rows / group + 1 + window;
+  int64_t tiles = (span + w.kt - 1) / w.kt + 1 + (sinks + w.kt - 1) / w.kt;
+  const int64_t every = (sk + w.kt - 1) / w.kt;
+  if (tiles > every) tiles = every;
+  const int64_t slots = (int64_t)device_cu_count() * (w.few ? 1 : 2);
+  int64_t parts = 1;
+  if (w.units < slots) {
+    parts = slots / w.units;
+    const int64_t most = tiles / 2;
+    if (parts > most) parts = most;
+    if (parts > 64) parts = 64;
+    if (parts < 1) parts = 1;
+  }
+  w.parts = (int)parts;
+  return w;
+}
+
+template <int D, int WR, int WK, int KW>
+static int launch_window(const WindowParams& p, hipStream_t s) {
+  const int64_t per = (int64_t)8 * p.chunk;
+  const int64_t grid = (p.n_items + per - 1) / per * per;
+  attn_window_kernel<D, WR, WK, KW><<<dim3((unsigned)grid), dim3(64 * WR * WK), 0, s>>>(p);
+  FDM_CHECK_LAUNCH();
+  return FDM_OK;
+}
+
+}  // namespace fdm
+
+using namespace fdm;
+
+extern "C" {
+
+int64_t fdm_attn_window_workspace_bytes(int64_t batch, int64_t sq, int64_t sk, int q_heads, int kv_heads, int head_dim, int64_t window, int64_t sinks) {
+  if (batch <= 0 || sq <= 0 || sk <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128) || window < 1 || sinks < 0) return 0;
+  const WindowPlan w = window_plan(batch, sq, sk, kv_heads, q_heads / kv_heads, head_dim, window < sk ? window : sk, sinks < sk ? sinks : sk);
+  return w.parts > 1 ? w.units * w.parts * w.rb_rows * (head_dim + 2) * 4 : 0;
+}
+
+int fdm_attn_window(void* o, const void* q, const void* k, const void* v, const int32_t* q_lens, const int32_t* kv_lens, int64_t batch, int64_t sq,
+                    int64_t sk, int q_heads, int kv_heads, int head_dim, int64_t q_batch_stride, int64_t q_tok_stride, int64_t k_batch_stride,
+                    int64_t k_tok_stride, int64_t v_batch_stride, int64_t v_tok_stride, int64_t o_batch_stride, int64_t o_tok_stride, float scale,
+                    int64_t window, int64_t sinks, void* workspace, int64_t workspace_bytes, fdm_stream_t stream) {
+  (void)hipGetLastError();  // drop any stale error of an earlier, unrelated runtime call: FDM_CHECK_LAUNCH must see only ours
+  if (batch < 0 || sq < 0 || sk < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || window < 1 || sinks < 0) return FDM_ERR_INVALID;
+  if (!(scale > 0.f) || scale > 3.0e38f) return FDM_ERR_INVALID;
+  if (head_dim != 64 && head_dim != 128) return FDM_ERR_UNSUPPORTED;
+  if (batch == 0 || sq == 0) return FDM_OK;
+  if (!o || !q || (sk > 0 && (!k || !v))) return FDM_ERR_INVALID;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
+  const int64_t strides = q_batch_stride | q_tok_stride | k_batch_stride | k_tok_stride | v_batch_stride | v_tok_stride | o_batch_stride | o_tok_stride;
+  if ((at & 15) || (strides & 7) || strides < 0) return FDM_ERR_INVALID;
+  if ((reinterpret_cast<uintptr_t>(q_lens) | reinterpret_cast<uintptr_t>(kv_lens)) & 3) return FDM_ERR_INVALID;
+  const int64_t group = q_heads / kv_heads;
+  // places, rows and items are 32-bit numbers in the kernel (addresses are 64-bit)
+  if (sk > (1 << 30) || sq > (1 << 30) || sq * group > (1 << 30) || batch > (1 << 24)) return FDM_ERR_UNSUPPORTED;
+  const int64_t win = window < sk ? window : (sk > 0 ? sk : 1), snk = sinks < sk ? sinks : sk;      // the same keys, and no overflow
+  const WindowPlan w = window_plan(batch, sq, sk, kv_heads, group, head_dim, win, snk);
+  const int64_t items = w.units * w.parts;
+  if (items > (1 << 28)) return FDM_ERR_UNSUPPORTED;
+  const int64_t need = w.parts > 1 ? w.units * w.parts * w.rb_rows * (head_dim + 2) * 4 : 0;
+  if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need)) return FDM_ERR_INVALID;
+  WindowParams p{};
+  p.o = (bf16_t*)o; p.q = (const bf16_t*)q; p.k = (const bf16_t*)k; p.v = (const bf16_t*)v; p.q_lens = q_lens; p.kv_lens = kv_lens;
+  p.q_bs = q_batch_stride; p.q_ts = q_tok_stride; p.k_bs = k_batch_stride; p.k_ts = k_tok_stride; p.v_bs = v_batch_stride; p.v_ts = v_tok_stride;
+  p.o_bs = o_batch_stride; p.o_ts = o_tok_stride;
+  p.batch = (int)batch; p.sq = (int)sq; p.sk = (int)sk; p.kv_heads = kv_heads; p.group = (int)group;
+  p.window = (int)win; p.sinks = (int)snk; p.n_blocks = (int)w.n_blocks; p.parts = w.parts; p.n_items = (int)items;
+  const int64_t each = (items + 7) / 8;
+  p.chunk = (int)(each < 32 ? each : 32);
+  p.scale_log2e = scale * 1.4426950408889634f;
+  p.ws_o = (float*)workspace;
+  p.ws_ml = p.ws_o + w.units * w.parts * w.rb_rows * head_dim;
+  hipStream_t s = to_stream(stream);
+  int rc;
+  if (head_dim == 128) rc = w.few ? launch_window<128, 1, 4, 32>(p, s) : launch_window<128, 4, 1, 64>(p, s);
+  else rc = w.few ? launch_window<64, 1, 4, 64>(p, s) : launch_window<64, 4, 1, 64>(p, s);
+  if (rc != FDM_OK || w.parts == 1) return rc;
+  const int64_t rows = batch * kv_heads * sq * group;
+  const int per_block = 256 / (head_dim / 4);
+  const unsigned grid = (unsigned)((rows + per_block - 1) / per_block);
+  if (head_dim == 128) attn_window_merge_kernel<128><<<dim3(grid), dim3(256), 0, s>>>(p, w.rb_rows);
+  else attn_window_merge_kernel<64><<<dim3(grid), dim3(256), 0, s>>>(p, w.rb_rows);
+  FDM_CHECK_LAUNCH();
+  return FDM_OK;
+}
+
+}  // extern "C"

@@ -14,7 +14,7 @@ mkdir -p "$OUT"
 OUT="$(cd "$OUT" && pwd)"
 HIPCC="${HIPCC:-/opt/rocm/bin/hipcc}"
 EXTRA="$*"
-UNITS="${FDM_BUILD_UNITS:-elementwise gemm attention decoder capi}"
+UNITS="${FDM_BUILD_UNITS:-elementwise gemm attention attention_window decoder capi}"
 [ -n "$FDM_BUILD_UNITS" ] && EXTRA="$EXTRA [units: $FDM_BUILD_UNITS]"
 [ -n "$FDM_SKIP_AUDIT" ] && EXTRA="$EXTRA [no audit]"
 EXTRA="${EXTRA# }"
@@ -55,8 +55,8 @@ for f in $UNITS; do
   extra=""
   [ "$f" = attention ] && extra="-fno-slp-vectorize -save-temps=obj"
   [ "$f" = gemm ] && extra="-save-temps=obj -Werror=inline-asm"     # (an asm clobber list naming a reserved register is an error)
-  # decoder: no packed-fp32 instructions (hipcc makes them of ordinary float code; some of their forms have given wrong results on these cards)
-  [ "$f" = decoder ] && extra="-Xclang -target-feature -Xclang -packed-fp32-ops"
+  # the decoder-side units: no packed-fp32 instructions (hipcc makes them of ordinary float code; some of their forms have given wrong results on these cards)
+  [ "$f" = decoder ] || [ "$f" = attention_window ] && extra="-Xclang -target-feature -Xclang -packed-fp32-ops"
   [ "$f" = capi ] && extra="-I$OUT -DFDM_HAVE_BUILD_INFO"
   "$HIPCC" $FLAGS $extra -c "$HERE/$f.hip" -o "$OUT/$f.o" &
   pids+=($!)

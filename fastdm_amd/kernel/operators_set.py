@@ -5,6 +5,7 @@ and returns None) and error behaviour (AssertionError for shape/dtype contract v
 reference's shims assert; RuntimeError for anything the native layer rejects, as TORCH_CHECK does).
 Single backend: every call goes through the C ABI; nothing here computes on the host.
 """
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -251,3 +252,43 @@ def sparse_scaled_dot_product_attention(query: torch.Tensor, key: torch.Tensor, 
     assert sparse_mask.dtype == torch.int8 and sparse_mask.is_contiguous()
     assert tuple(sparse_mask.shape) == (B, num_q_heads, nq, nk), f"sparse_mask must be {(B, num_q_heads, nq, nk)}"
     return _attn(query, key, value, num_q_heads, num_kv_heads, head_dim, is_causal, scale, sparse_mask, SPARSE_BLOCK_Q, SPARSE_BLOCK_K)
+
+
+def window_scaled_dot_product_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                                        window: int, sinks: int = 0, scale: Optional[float] = None, q_lens: Optional[torch.Tensor] = None,
+                                        kv_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention whose queries see the last `window` keys (their own among them) and the first `sinks`: query [B, Sq, Hq*D], key / value
+    [B, Sk, Hkv*D] (a cache, or slices of one: any batch and token strides), [B, Sq, Hq*D] out.  The queries of a sequence are the last of its tokens:
+    row t is at place kv_len - q_len + t and sees key j iff j <= place and (place - j < window or j < sinks).  q_lens / kv_lens: int32 [B] on the GPU
+    for padded batches and part-filled caches (default Sq / Sk; lengths outside 0 .. Sq / Sk count as the nearest).  Rows past q_len and rows that see
+    nothing are zeros; keys past kv_len and keys no row sees may hold anything.  Prompts, chunks behind a cache, and single tokens (Sq = 1)."""
+    N.need_gpu("window_scaled_dot_product_attention", query, key, value, q_lens, kv_lens)
+    assert query.dtype == BF16 and key.dtype == BF16 and value.dtype == BF16, "window_scaled_dot_product_attention: bf16 only"
+    assert query.ndim == 3 and key.ndim == 3 and key.shape == value.shape, "window_scaled_dot_product_attention: [B, S, heads * head_dim]"
+    B, Sq, width = query.shape
+    Sk = key.shape[1]
+    assert head_dim in (64, 128), "window_scaled_dot_product_attention: head_dim 64 or 128"
+    assert num_kv_heads > 0 and num_q_heads % num_kv_heads == 0, "window_scaled_dot_product_attention: q heads are a multiple of the kv heads"
+    assert width == num_q_heads * head_dim and key.shape[2] == num_kv_heads * head_dim and key.shape[0] == B, "window_scaled_dot_product_attention: shapes"
+    assert window >= 1 and sinks >= 0, "window_scaled_dot_product_attention: window >= 1, sinks >= 0"
+    for t in (query, key, value):
+        assert t.stride(2) == 1, "window_scaled_dot_product_attention: tokens must be dense"
+    for lens in (q_lens, kv_lens):
+        assert lens is None or (lens.dtype == torch.int32 and lens.shape == (B,) and lens.is_contiguous()), "window_scaled_dot_product_attention: lengths int32 [B]"
+    if scale is None:
+        scale = head_dim ** -0.5
+    assert 0.0 < scale < 3e38, "window_scaled_dot_product_attention: scale > 0"
+    out = torch.empty((B, Sq, width), device=query.device, dtype=BF16)
+    need = _window_workspace(B, Sq, Sk, num_q_heads, num_kv_heads, head_dim, window, sinks)
+    ws = torch.empty(need, device=query.device, dtype=torch.uint8) if need else None      # of this call alone: a captured graph's comes from its own pool
+    (q_bs, q_ts, _), (k_bs, k_ts, _), (v_bs, v_ts, _) = query.stride(), key.stride(), value.stride()
+    with N.on_device(query):
+        N.check(N.lib().fdm_attn_window(N.ptr(out), N.ptr(query), N.ptr(key), N.ptr(value), N.ptr(q_lens), N.ptr(kv_lens), B, Sq, Sk, num_q_heads,
+                                        num_kv_heads, head_dim, q_bs, q_ts, k_bs, k_ts, v_bs, v_ts, Sq * width, width, scale, window, sinks, N.ptr(ws), need,
+                                        N.stream(query.device.index)), "window_scaled_dot_product_attention")
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _window_workspace(*shape) -> int:
+    return int(N.lib().fdm_attn_window_workspace_bytes(*shape))

@@ -465,6 +465,20 @@ int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, c
                        int64_t qo_batch_stride, int64_t qo_tok_stride, int64_t ko_batch_stride, int64_t ko_tok_stride, float amplitude,
                        int is_neox, fdm_stream_t stream);
 
+/* Causal attention with a sliding window and sinks (ABI 21): prompts, chunks of a prompt behind a cache, single tokens.
+ *   q [batch, sq, q_heads * head_dim], k / v [batch, sk, kv_heads * head_dim], o as q; bf16, batch and token strides in elements (multiples of 8, 16-byte
+ *   aligned tensors); q_heads a multiple of kv_heads; head_dim 64 or 128.
+ *   q_lens, kv_lens: int32 [batch] on the device, or NULL for sq / sk (values outside 0 .. sq / sk count as the nearest).  The queries of a sequence are
+ *   the last q_len of its kv_len tokens: row t < q_len is at place kv_len - q_len + t and sees key j iff j <= place and (place - j < window or j < sinks).
+ *   Rows at or past q_len, and rows that see nothing, are zeros.  Keys at or past kv_len are not read; what a row does not see does not reach it, NaNs
+ *   and infinities included.  softmax(q k^T * scale) v with fp32 statistics, scale > 0; window >= 1 (>= sk: plain causal), sinks >= 0.
+ * workspace: 16-byte aligned, >= fdm_attn_window_workspace_bytes(...) of the same arguments (0: none), rewritten by every call.                */
+int64_t fdm_attn_window_workspace_bytes(int64_t batch, int64_t sq, int64_t sk, int q_heads, int kv_heads, int head_dim, int64_t window, int64_t sinks);
+int fdm_attn_window(void* o, const void* q, const void* k, const void* v, const int32_t* q_lens, const int32_t* kv_lens, int64_t batch, int64_t sq,
+                    int64_t sk, int q_heads, int kv_heads, int head_dim, int64_t q_batch_stride, int64_t q_tok_stride, int64_t k_batch_stride,
+                    int64_t k_tok_stride, int64_t v_batch_stride, int64_t v_tok_stride, int64_t o_batch_stride, int64_t o_tok_stride, float scale,
+                    int64_t window, int64_t sinks, void* workspace, int64_t workspace_bytes, fdm_stream_t stream);
+
 /* TeaCache metric (caching/xcaching.py:214): out[0] = sum|a-b|, out[1] = sum|b| (fp32 atomics;
  * caller zeroes out[0..1]).                                                                      */
 int fdm_absdiff_sums(float* out2, const void* a, const void* b, int64_t n, fdm_stream_t stream);

@@ -101,3 +101,35 @@ def test_wavelength_blends_between_its_two_ends():
 def test_frequencies_refuse(kw):
     with pytest.raises(ValueError):
         RotaryFrequencies(**kw)
+
+
+def c_window(**kw):
+    a = dict(o=4096, q=8192, k=12288, v=16384, ql=None, kl=None, B=1, sq=4, sk=8, hq=2, hk=1, D=64, qbs=512, qts=128, kbs=512, kts=64, vbs=512, vts=64, obs=512, ots=128,
+             scale=0.125, window=4, sinks=0, ws=None, wsb=0)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return N.lib().fdm_attn_window(a["o"], a["q"], a["k"], a["v"], a["ql"], a["kl"], a["B"], a["sq"], a["sk"], a["hq"], a["hk"], a["D"], a["qbs"], a["qts"], a["kbs"], a["kts"],
+                                   a["vbs"], a["vts"], a["obs"], a["ots"], a["scale"], a["window"], a["sinks"], a["ws"], a["wsb"], None)
+
+
+@pytest.mark.parametrize("kw,code", [(dict(o=None), -1), (dict(q=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(q=8200), -1), (dict(kts=63), -1), (dict(vbs=-512), -1),
+                                     (dict(ql=2), -1), (dict(kl=6), -1), (dict(hq=3, hk=2), -1), (dict(hk=0), -1), (dict(window=0), -1), (dict(sinks=-1), -1),
+                                     (dict(scale=0.0), -1), (dict(scale=-1.0), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(B=-1), -1),
+                                     (dict(D=96), -2), (dict(sk=1 << 31), -2), (dict(sq=1 << 31), -2), (dict(sq=0, q=None), 0), (dict(B=0, o=None), 0),
+                                     (dict(sq=1, sk=100000, window=100000), -1), (dict(sq=1, sk=100000, window=100000, ws=64, wsb=64), -1)])
+def test_window_attention_c_entry_refuses(kw, code):
+    assert c_window(**kw) == code
+
+
+def test_window_attention_workspace_is_for_few_long_rows_alone():
+    need = N.lib().fdm_attn_window_workspace_bytes
+    assert need(1, 1, 100000, 8, 8, 128, 100000, 0) > 0
+    assert need(64, 1, 100, 8, 8, 128, 100, 0) == 0 and need(1, 65536, 65536, 32, 8, 128, 4096, 4) == 0
+    assert need(0, 1, 1, 1, 1, 64, 1, 0) == 0 and need(1, 1, 1, 3, 2, 64, 1, 0) == 0
+
+
+def test_window_attention_refuses_cpu_tensors():
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention
+    x = torch.zeros(1, 4, 64, dtype=BF16)
+    with pytest.raises(RuntimeError, match="GPU"):
+        window_scaled_dot_product_attention(x, x, x, 1, 1, 64, 2)

@@ -234,3 +234,227 @@ def test_rotary_positions_of_no_tokens():
     freqs = RotaryFrequencies(64, device="cuda")
     q, k = rotary_positions(torch.empty(2, 0, 128, device="cuda", dtype=BF16), torch.empty(2, 0, 64, device="cuda", dtype=BF16), 64, freqs)
     assert q.shape == (2, 0, 128) and k.shape == (2, 0, 64)
+
+
+# ================================================================================================ window_scaled_dot_product_attention
+def window64(q, k, v, Hq, Hk, D, window, sinks, scale=None, q_lens=None, kv_lens=None):
+    """In 64 bits, one sequence and kv head at a time, over the visible keys alone; and the tolerance element by element."""
+    B, S, _ = q.shape
+    L = k.shape[1]
+    scale = D ** -0.5 if scale is None else scale
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    G = Hq // Hk
+    for b in range(B):
+        qn = S if q_lens is None else min(max(int(q_lens[b]), 0), S)
+        kn = L if kv_lens is None else min(max(int(kv_lens[b]), 0), L)
+        if qn == 0 or kn == 0:
+            continue
+        place = (kn - qn + torch.arange(qn, device=q.device))[:, None]
+        j = torch.arange(kn, device=q.device)[None]
+        see = (j <= place) & ((place - j < window) | (j < sinks))
+        for hk in range(Hk):
+            kk, vv = k[b, :kn, hk * D:(hk + 1) * D].double(), v[b, :kn, hk * D:(hk + 1) * D].double()
+            some = see.any(0)                                # what nobody sees may be anything: left out of the products
+            kk, vv = kk[some], vv[some]
+            sub = see[:, some]
+            for g in range(G):
+                at = slice((hk * G + g) * D, (hk * G + g + 1) * D)
+                qq = q[b, :qn, at].double()
+                s = ((qq @ kk.t()) * scale).masked_fill(~sub, -math.inf)
+                any_ = sub.any(1, keepdim=True)
+                p = torch.where(any_, torch.softmax(s, -1), torch.zeros_like(s))
+                o, size = p @ vv, p @ vv.abs()
+                # scores: D products summed in fp32, scaled and shifted (each step 2^-24 of the sum of magnitudes); 2^x to 2^-22.  A weight and the weights'
+                # sum are off by that, relative; the weight is rounded to bf16, and the result once more
+                delta = (D + 4) * 2.0 ** -24 * scale * ((qq.abs() @ kk.abs().t()) * sub).amax(1, keepdim=True)
+                out[b, :qn, at] = o
+                tol[b, :qn, at] = o.abs() * HALF_STEP + size * (HALF_STEP + 2 * delta + 2.0 ** -20) * (1 + HALF_STEP)
+    return out, tol
+
+
+def check_window(q, k, v, Hq, Hk, D, window, sinks, what="window", **kw):
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention
+    got = window_scaled_dot_product_attention(q, k, v, Hq, Hk, D, window, sinks=sinks, **kw)
+    want, tol = window64(q, k, v, Hq, Hk, D, window, sinks, **kw)
+    assert_within(got, want, tol, what)
+    return got
+
+
+def lens(*n):
+    return torch.tensor(n, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,L,window,sinks", [(1, 1, 1, 0), (1, 1, 4, 3), (2, 2, 1, 0), (5, 5, 2, 1), (63, 63, 7, 0), (64, 64, 64, 4), (65, 65, 16, 2), (200, 200, 1000, 0),
+                                              (130, 130, 1, 1), (257, 257, 64, 64), (300, 300, 33, 130), (129, 500, 100, 5), (1, 700, 65, 3), (3, 333, 40, 129),
+                                              (8, 1025, 256, 0), (1, 4100, 4096, 4), (700, 700, 128, 10), (31, 2000, 500, 1), (513, 1025, 300, 7)])
+def test_window_attention(S, L, window, sinks, D):
+    g = gen(S * 7 + L + window + sinks + D)
+    for B, Hq, Hk in ((1, 4, 4), (2, 8, 2), (1, 7, 1), (3, 3, 3)):
+        q, k, v = randn(g, B, S, Hq * D, scale=2.0), randn(g, B, L, Hk * D), randn(g, B, L, Hk * D)
+        check_window(q, k, v, Hq, Hk, D, window, sinks)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,L,window,sinks", [(150, 150, 40, 3), (150, 400, 64, 70), (1, 900, 100, 2), (4, 900, 600, 1)])
+def test_window_attention_of_ragged_batches(S, L, window, sinks, D):
+    """Padded batches and part-filled caches, empty sequences, more queries than tokens (rows that see nothing), lengths out of range."""
+    g = gen(S + L + D)
+    B, Hq, Hk = 6, 6, 2
+    q, k, v = randn(g, B, S, Hq * D), randn(g, B, L, Hk * D), randn(g, B, L, Hk * D)
+    kv = lens(L, L // 2, 1, 0, max(1, S // 2), L + 50)
+    qn = lens(S, S // 2, 1, S, S, 2 * S)
+    check_window(q, k, v, Hq, Hk, D, window, sinks, kv_lens=kv)
+    check_window(q, k, v, Hq, Hk, D, window, sinks, q_lens=qn)
+    got = check_window(q, k, v, Hq, Hk, D, window, sinks, q_lens=qn, kv_lens=kv)
+    assert (got[3] == 0).all() and (got[1, S // 2:] == 0).all()                # an empty sequence; rows past the queries
+    negative = lens(-3, S, S, S, S, S)
+    assert (check_window(q, k, v, Hq, Hk, D, window, sinks, q_lens=negative)[0] == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_window_attention_on_slices_of_a_projection_and_a_cache(D):
+    """q from a fused projection; k and v from caches with other orders of the axes, and one sequence's cache shared by the whole batch."""
+    g = gen(D)
+    B, S, L, Hq, Hk = 3, 70, 260, 4, 2
+    qkv = randn(g, B, S, (Hq + 2 * Hk) * D + 8)
+    q = qkv[..., 8:8 + Hq * D]
+    cache = randn(g, L + 40, B, 2, Hk * D)                                     # token-major, k and v side by side
+    k, v = cache[10:10 + L, :, 0].transpose(0, 1), cache[10:10 + L, :, 1].transpose(0, 1)
+    plain = check_window(q.contiguous(), k.contiguous(), v.contiguous(), Hq, Hk, D, 50, 5)
+    assert torch.equal(check_window(q, k, v, Hq, Hk, D, 50, 5), plain)
+    shared = k[:1].expand(B, L, Hk * D)
+    assert torch.equal(check_window(q, shared, v, Hq, Hk, D, 50, 5), check_window(q, shared.contiguous(), v, Hq, Hk, D, 50, 5))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,L", [(1, 400), (5, 400), (90, 400), (300, 300)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_window_attention_keeps_what_is_not_seen_out(S, L, bad, D):
+    """Keys past the lengths, keys in front of every window and behind the sinks hold anything; a value some rows see reaches those rows alone."""
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    g = gen(S + D)
+    B, Hq, Hk, window, sinks = 2, 6, 2, 37, 3
+    q, k, v = randn(g, B, S, Hq * D), randn(g, B, L, Hk * D), randn(g, B, L, Hk * D)
+    kv = lens(L - 30, L)
+    qn = lens(min(S, L - 30), S)
+    clean = check_window(q, k, v, Hq, Hk, D, window, sinks, q_lens=qn, kv_lens=kv)
+    k2, v2 = k.clone(), v.clone()
+    k2[0, L - 30:], v2[0, L - 30:] = bad, bad
+    for b, (n, t) in enumerate(((L - 30, min(S, L - 30)), (L, S))):
+        front = max(sinks, n - t - window + 1)
+        k2[b, sinks:front], v2[b, sinks:front] = bad, bad
+    assert torch.equal(attend(q, k2, v2, Hq, Hk, D, window, sinks=sinks, q_lens=qn, kv_lens=kv), clean)
+    if S > 1:
+        # a bad value inside: key j of sequence 1, seen by the rows at places j .. j + window - 1
+        j = L - S // 2 - 1
+        v3 = v.clone()
+        v3[1, j] = bad
+        got = attend(q, k, v3, Hq, Hk, D, window, sinks=sinks, q_lens=qn, kv_lens=kv)
+        place = torch.arange(L - S, L, device="cuda")
+        sees = (place >= j) & (place < j + window)
+        assert torch.equal(got[1, ~sees], clean[1, ~sees]) and torch.equal(got[0], clean[0])
+        assert not torch.isfinite(got[1, sees]).any()
+        k3 = k.clone()
+        k3[1, j] = bad
+        got = attend(q, k3, v, Hq, Hk, D, window, sinks=sinks, q_lens=qn, kv_lens=kv)
+        assert torch.equal(got[1, ~sees], clean[1, ~sees])
+
+
+def test_window_attention_scores_of_every_size():
+    """Large, small and equal scores: the running maximum moves, stays, and starts far below."""
+    g = gen(9)
+    D, S = 64, 200
+    for scale, offset in ((50.0, 0.0), (1e-6, 0.0), (1.0, 0.0), (1.0, 1e4), (1.0, -1e4)):
+        q, k, v = randn(g, 1, S, 2 * D), randn(g, 1, S, 2 * D), randn(g, 1, S, 2 * D)
+        if offset:
+            q[..., 0], k[..., 0] = 100.0, offset
+            q[..., D], k[..., D] = 100.0, offset
+        check_window(q, k, v, 2, 2, D, 64, 4, scale=scale * D ** -0.5)
+    one = torch.zeros(1, S, 2 * D, device="cuda", dtype=BF16)
+    check_window(one, one, randn(g, 1, S, 2 * D), 2, 2, D, 64, 4)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_window_attention_with_an_open_window_is_causal_attention(D):
+    from fastdm_amd.kernel.operators_set import scaled_dot_product_attention
+    g = gen(D + 1)
+    S, H = 333, 3
+    q, k, v = randn(g, 1, S, H * D), randn(g, 1, S, H * D), randn(g, 1, S, H * D)
+    got = check_window(q, k, v, H, H, D, 1 << 40, 0)
+    want, tol = window64(q, k, v, H, H, D, S, 0)
+    assert_within(scaled_dot_product_attention(q, k, v, H, H, D, is_causal=True), want, tol, "causal")
+    assert_within(got, want, tol, "open window")
+
+
+def test_window_attention_parts_agree_with_whole_lists():
+    """The same token attended alone (its tiles in parts, merged) and as the last row of a long batch of tokens (whole lists)."""
+    g = gen(11)
+    D, Hq, Hk, L = 128, 8, 2, 5000
+    q, k, v = randn(g, 1, L, Hq * D), randn(g, 1, L, Hk * D), randn(g, 1, L, Hk * D)
+    whole = check_window(q[:, -600:], k, v, Hq, Hk, D, 3000, 9)
+    for n in (1, 2, 8, 9, 40):
+        part = check_window(q[:, -n:].contiguous(), k, v, Hq, Hk, D, 3000, 9)
+        want, tol = window64(q[:, -n:], k, v, Hq, Hk, D, 3000, 9)
+        assert ((part.double() - whole[:, -n:].double()).abs() <= 2 * tol).all()
+
+
+def test_window_attention_repeats_bit_for_bit_on_streams_and_in_graphs():
+    """Two captured graphs, replayed in turn with eager calls between, and calls on two streams at once: each its own workspace."""
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    g = gen(12)
+    D, Hq, Hk, L = 128, 8, 2, 6000
+    sets = [(randn(g, 2, 1, Hq * D), randn(g, 2, L, Hk * D), randn(g, 2, L, Hk * D)) for _ in range(2)]
+    kv = [lens(L, L - 777), lens(L - 1, 4000)]
+    want = [attend(*s, Hq, Hk, D, 4000, sinks=4, kv_lens=n) for s, n in zip(sets, kv)]
+    assert not torch.equal(want[0], want[1])
+    graphs, outs = [], []
+    for s, n in zip(sets, kv):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(attend(*s, Hq, Hk, D, 4000, sinks=4, kv_lens=n))
+        graphs.append(graph)
+    for _ in range(4):
+        for i in (0, 1):
+            outs[i].zero_()
+            graphs[i].replay()
+            assert torch.equal(attend(*sets[1 - i], Hq, Hk, D, 4000, sinks=4, kv_lens=kv[1 - i]), want[1 - i])
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], want[i])
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = attend(*sets[i], Hq, Hk, D, 4000, sinks=4, kv_lens=kv[i])
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_window_attention_of_nothing():
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    e = lambda *s: torch.empty(*s, device="cuda", dtype=BF16)  # noqa: E731
+    assert attend(e(0, 4, 128), e(0, 4, 128), e(0, 4, 128), 2, 2, 64, 4).shape == (0, 4, 128)
+    assert attend(e(2, 0, 128), e(2, 4, 128), e(2, 4, 128), 2, 2, 64, 4).shape == (2, 0, 128)
+    q = torch.ones(2, 3, 128, device="cuda", dtype=BF16)
+    assert (attend(q, e(2, 0, 128), e(2, 0, 128), 2, 2, 64, 4) == 0).all()     # no keys: rows that see nothing
+
+
+def test_window_attention_behind_offsets_over_32_bits():
+    """A cache of more than 2^32 elements: the last sequence's keys lie past every 32-bit offset."""
+    D, Hk, Hq, B, L = 128, 8, 8, 5, 1 << 20
+    if torch.cuda.mem_get_info()[0] < 48 << 30:
+        pytest.skip("needs 48 GB")
+    k = torch.zeros(B, L, Hk * D, device="cuda", dtype=BF16)
+    v = torch.zeros(B, L, Hk * D, device="cuda", dtype=BF16)
+    assert k.numel() > 1 << 32
+    g = gen(13)
+    q = randn(g, B, 1, Hq * D)
+    k[:, -600:], v[:, -600:] = randn(g, B, 600, Hk * D), randn(g, B, 600, Hk * D)
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    got = attend(q, k, v, Hq, Hk, D, 500)
+    want, tol = window64(q, k[:, -600:], v[:, -600:], Hq, Hk, D, 500, 0)
+    assert_within(got, want, tol, "far keys")
