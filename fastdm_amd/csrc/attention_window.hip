@@ -15,8 +15,10 @@
 //   waves     WR waves over rows (32 each) times WK waves over the keys of a tile: prompts WK = 1; few rows (single tokens) WR = 1, WK = 4, merged
 //             through LDS at the end.  Where the blocks would not fill the chip, a block's tile list is cut into parts that run side by side and
 //             are merged by a second small launch.
-//   NaN       what a row does not see does not reach it: masked scores are replaced, keys past kv_len are never read, and where a masked tile holds a
-//             value that is not finite (0 * NaN is NaN in the matrix core) the product is taken token by token with the invisible values zeroed.
+//   NaN       what a row does not see does not reach it, though 0 * NaN is NaN in the matrix core: masked scores are replaced, keys past kv_len are never
+//             read, values that no row of the block sees are zeroed in LDS, and a block that finds one that is not finite among those that only some
+//             rows see starts over: product with the finite values, and a second product of marks for the rows that see one that is not.
+#include <type_traits>
 #include "common.h"
 #include "attn_common.h"
 
@@ -111,29 +113,38 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
     for (int ks = 0; ks < KSTEPS; ++ks) qf[ks] = *reinterpret_cast<const i32x4*>(qp + 16 * ks);
   }
 
-  // ---- K / V staging by LDS-DMA: lane-linear destination, the swizzle is applied to the source
-  int srow[LD];
-  int kch[LD], vch[LD];
+  // ---- K / V staging by LDS-DMA: lane-linear destination, the swizzle is applied to the source.  A piece is a wave-uniform tile base plus a 32-bit
+  //      lane offset that stays.  The DMA is an asm statement (it writes no register): hipcc puts s_waitcnt vmcnt(0) in front of LDS reads that
+  //      follow its builtin, which is the next tile's DMA here; the waits are the two lines at the top of the loop.
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem + wave * 1024;
+  uint32_t kofs[LD], vofs[LD];
 #pragma unroll
   for (int i = 0; i < LD; ++i) {
-    const int slot = tid + i * NT;
-    srow[i] = slot / CPR;
-    kch[i] = Swz<D>::k(srow[i], slot % CPR) * 8;
-    vch[i] = Swz<D>::v(srow[i], slot % CPR) * 8;
+    const int slot = tid + i * NT, r = slot / CPR;
+    kofs[i] = (uint32_t)(r * (int)p.k_ts * 2 + Swz<D>::k(r, slot % CPR) * 16);
+    vofs[i] = (uint32_t)(r * (int)p.v_ts * 2 + Swz<D>::v(r, slot % CPR) * 16);
   }
+  auto dma = [&](const bf16_t* base, uint32_t ofs, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(ofs), "s"(base) : "memory");
+  };
   auto stage = [&](int t, int buf) {
-    uint8_t* sk_ = smem + buf * 2 * TILE_BYTES + wave * 1024;
-    uint8_t* sv_ = sk_ + TILE_BYTES;
+    const uint32_t lds = lds0 + buf * 2 * TILE_BYTES;
     const int last = kv_len - 1 - t * KT;       // >= 0: a listed tile holds a visible key
     const bf16_t* kt_ = kbase + (int64_t)t * KT * p.k_ts;
     const bf16_t* vt_ = vbase + (int64_t)t * KT * p.v_ts;
+    if (last >= KT - 1) {
 #pragma unroll
-    for (int i = 0; i < LD; ++i) {
-      const int r = min(srow[i], last);         // past the sequence: its last key again (masked)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kt_ + (int64_t)r * p.k_ts + kch[i]),
-                                       (__attribute__((address_space(3))) void*)(sk_ + i * (NT * 16)), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vt_ + (int64_t)r * p.v_ts + vch[i]),
-                                       (__attribute__((address_space(3))) void*)(sv_ + i * (NT * 16)), 16, 0, 0);
+      for (int i = 0; i < LD; ++i) {
+        dma(kt_, kofs[i], lds + i * (NT * 16));
+        dma(vt_, vofs[i], lds + TILE_BYTES + i * (NT * 16));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < LD; ++i) {            // past the sequence: its last key again (masked)
+        const int r = (tid + i * NT) / CPR, over = max(r - last, 0);
+        dma(kt_, kofs[i] - (uint32_t)(over * (int)p.k_ts * 2), lds + i * (NT * 16));
+        dma(vt_, vofs[i] - (uint32_t)(over * (int)p.v_ts * 2), lds + TILE_BYTES + i * (NT * 16));
+      }
     }
   };
 
@@ -152,9 +163,13 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
   for (int d = 0; d < DT; ++d)
     vld[d] = TILE_BYTES + (wk * KW + 4 * h + tq) * ROWB + (uint32_t)Swz<D>::v(4 * h + tq, d * 4 + 2 * (gi & 1) + (tp >> 1)) * 16 + 8 * (tp & 1);
 
-  // one key tile for this wave; base: place of its first key.  MASK: some row of the wave does not see some key
-  auto process = [&](auto mask_c, int base, uint32_t buf) {
-    constexpr bool MASK = decltype(mask_c)::value;
+  // key kk of a tile whose first key is `hi` in front of the row's place: 0 <= hi - kk < window, or a sink (`sink` <= hi + 1).  No branch: | and not ||
+  auto sees = [&](int hi, int sink, int kk) { return ((unsigned)(hi - kk) < (unsigned)p.window) | (kk < sink); };
+
+  // one key tile for this wave; base: place of its first key.  KIND 0: every row sees every key, 1: masked, 2: masked, values that are not finite apart
+  auto process = [&](auto kind_c, int base, uint32_t buf) {
+    constexpr int KIND = decltype(kind_c)::value;
+    constexpr bool MASK = KIND != 0;
     const uint8_t* sb = smem + buf;
     f32x16 s[NKT];
 #pragma unroll
@@ -170,13 +185,13 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
       }
     if constexpr (MASK) {
       const int at = base + 4 * h;              // element e of tile n is key at + 32 n + (e & 3) + 8 (e >> 2)
-      const int hi = place - at, lo = place - p.window - at, sink = p.sinks - at;
+      const int hi = place - at, sink = min(p.sinks - at, hi + 1);
 #pragma unroll
       for (int n = 0; n < NKT; ++n)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int kk = n * 32 + (e & 3) + 8 * (e >> 2);
-          if (!(kk <= hi && (kk > lo || kk < sink))) s[n][e] = -INFINITY;
+          s[n][e] = sees(hi, sink, kk) ? s[n][e] : -INFINITY;
         }
     }
     // row maximum: med3(a, b, +inf) is max without the canonicalisation hipcc puts in front of fmaxf
@@ -216,72 +231,109 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
       const uint8_t* a = sb + vld[d] + (n * 32 + 16 * u) * ROWB;      // keys 4 h + tq, and 8 further
       return tr_pair(a, a + 8 * ROWB);
     };
-    if constexpr (MASK) {
-      // a masked weight is 0, and 0 * NaN is NaN: look for values that are not finite (exponent all ones)
-      u16x2 top = {0, 0};
-#pragma unroll
-      for (int n = 0; n < NKT; ++n)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const i32x4 f = vfrag(n, u, d);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, f[w] & 0x7fff7fff));
-          }
-      if (__any(top[0] >= 0x7f80 || top[1] >= 0x7f80)) {
-        for (int t = wt_lo; t <= wt_hi; ++t) {       // token by token, what it does not see zeroed
-          const int at = base + 4 * h;
-          const int hi = first + t - at, lo = hi - p.window, sink = p.sinks - at;
-          const bool mine = tok == t;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            f32x16 add = oacc[d];       // the same sums in the same order as below: the same bits
-#pragma unroll
-            for (int n = 0; n < NKT; ++n)
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                i32x4 f = vfrag(n, u, d);
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                  const int k0 = n * 32 + 16 * u + 8 * (w >> 1) + 2 * (w & 1);
-                  const bool see0 = k0 <= hi && (k0 > lo || k0 < sink), see1 = k0 + 1 <= hi && (k0 + 1 > lo || k0 + 1 < sink);
-                  f[w] &= (see0 ? 0x0000ffff : 0) | (see1 ? (int)0xffff0000 : 0);
-                }
-                add = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, pf[n][u]), add, 0, 0, 0);
-              }
-            if (mine) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) oacc[d][e] = add[e];
-            }
-          }
-        }
-        return;
-      }
-    }
 #pragma unroll
     for (int n = 0; n < NKT; ++n)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
+        i32x4 see;                              // KIND 2: 1.0 where the row sees the key, laid out as P
+        if constexpr (KIND == 2) {
+          const int hi = place - base - 4 * h, sink = min(p.sinks - base - 4 * h, hi + 1);
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-          oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vfrag(n, u, d)), __builtin_bit_cast(bf16x8, pf[n][u]), oacc[d], 0, 0, 0);
+          for (int w = 0; w < 4; ++w) {
+            const int k0 = n * 32 + 16 * u + 8 * (w >> 1) + 2 * (w & 1);
+            see[w] = (sees(hi, sink, k0) ? 0x3f80 : 0) | (sees(hi, sink, k0 + 1) ? 0x3f800000 : 0);
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          i32x4 f = vfrag(n, u, d);
+          if constexpr (KIND == 2) {
+            i32x4 mark;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const bool b0 = (f[w] & 0x7f80) == 0x7f80, b1 = (f[w] & 0x7f800000) == 0x7f800000;
+              mark[w] = (b0 ? 0x3f80 : 0) | (b1 ? 0x3f800000 : 0);
+              f[w] &= ~((b0 ? 0xffff : 0) | (b1 ? (int)0xffff0000 : 0));
+            }
+            f32x16 count;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) count[e] = 0.f;
+            count = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, mark), __builtin_bit_cast(bf16x8, see), count, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) oacc[d][e] = count[e] > 0.f ? __builtin_nanf("") : oacc[d][e];
+          }
+          oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f), __builtin_bit_cast(bf16x8, pf[n][u]), oacc[d], 0, 0, 0);
+          if constexpr (KIND == 2) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
   };
 
-  if (i_begin < i_end) stage(tile_at(i_begin), 0);
-  uint32_t buf = 0;
-  for (int i = i_begin; i < i_end; ++i) {
+  // ---- the list in three stretches: [sinks, the window's lower edge) masked, [mid_lo, mid_hi) seen whole by every row of the block, the diagonal masked
+  //      (one loop with both bodies in it costs more registers than the kernel has)
+  int mid_lo = n_sink, mid_hi = n_sink;
+  if (n_list > 0) {
+    const int under = first + bt_hi - p.window;                    // the last key that some row does not see below its window
+    const int t_lo = under >= 0 ? under / KT + 1 : 0, t_hi = max(0, first + bt_lo + 1) / KT;
+    mid_lo = min(n_sink + max(t_lo - w_begin, 0), n_list);
+    mid_hi = max(min(n_sink + t_hi - w_begin, n_list), mid_lo);
+  }
+  const bool has_rows = wt_lo <= wt_hi;
+  // a masked tile's values, each thread its own pieces: zeroes for keys that no row of the block sees; the largest magnitude of the others is kept
+  u16x2 top = {0, 0};
+  const int bp_lo = first + bt_lo, bp_hi = first + bt_hi;
+  auto clean = [&](int base, int buf) {
+    uint8_t* sv = smem + buf * 2 * TILE_BYTES + TILE_BYTES + tid * 16;
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+      const int key = base + (tid + j * NT) / CPR;
+      i32x4* piece = reinterpret_cast<i32x4*>(sv + j * (NT * 16));
+      if ((key > bp_hi) | ((key <= bp_lo - p.window) & (key >= p.sinks))) {
+        *piece = i32x4{0, 0, 0, 0};
+      } else {
+        const i32x4 f = *piece;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, f[w] & 0x7fff7fff));
+      }
+    }
+  };
+  int buf = 0, i = i_begin;
+  auto arrive = [&](bool masked) {                      // tile i is there, tile i + 1 on its way
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // this wave's pieces of tile i have landed ...
+    if (masked) clean(tile_at(i) * KT, buf);
     __syncthreads();                                    // ... and everybody's; the other buffer has been read
     if (i + 1 < i_end) stage(tile_at(i + 1), buf ^ 1);
-    const int base = tile_at(i) * KT + wk * KW;
-    const bool none = wt_lo > wt_hi || base > wp_hi || (base + KW <= wp_lo - p.window + 1 && base >= p.sinks);
-    if (!none) {
-      const bool all = base + KW - 1 <= wp_lo && (base > wp_hi - p.window || base + KW <= p.sinks);
-      if (all) process(std::false_type{}, base, buf * 2 * TILE_BYTES);
-      else process(std::true_type{}, base, buf * 2 * TILE_BYTES);
+  };
+  if (i_begin < i_end) stage(tile_at(i_begin), 0);
+  for (int stretch = 0; stretch < 3; ++stretch) {
+    const int to = min(stretch == 0 ? mid_lo : stretch == 1 ? mid_hi : n_list, i_end);
+    if (stretch == 1) {
+      for (; i < to; ++i, buf ^= 1) {
+        arrive(false);
+        if (has_rows) process(std::integral_constant<int, 0>{}, 0, buf * 2 * TILE_BYTES);
+      }
+    } else {
+      for (; i < to; ++i, buf ^= 1) {
+        arrive(true);
+        const int base = tile_at(i) * KT + wk * KW;
+        if (has_rows && base <= wp_hi && (base + KW > wp_lo - p.window + 1 || base < p.sinks)) process(std::integral_constant<int, 1>{}, base, buf * 2 * TILE_BYTES);
+      }
     }
-    buf ^= 1;
+  }
+  if (__syncthreads_or((top[0] >= 0x7f80) | (top[1] >= 0x7f80))) {      // (exponent all ones) once more from the start, with care
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) oacc[d][e] = 0.f;
+    m_run = -3.0e38f;
+    l_run = 0.f;
+    buf = 0;
+    i = i_begin;
+    if (i_begin < i_end) stage(tile_at(i_begin), 0);
+    for (; i < i_end; ++i, buf ^= 1) {
+      arrive(true);
+      const int base = tile_at(i) * KT + wk * KW;
+      if (has_rows && base <= wp_hi && (base + KW > wp_lo - p.window + 1 || base < p.sinks)) process(std::integral_constant<int, 2>{}, base, buf * 2 * TILE_BYTES);
+    }
   }
 
   float l_tot = l_run + __shfl_xor(l_run, 32, 64);
@@ -301,18 +353,17 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
       }
       return;
     }
-    const float inv = live && l_tot != 0.f ? 1.0f / l_tot : 0.f;
+    const int keep = live && l_tot != 0.f ? -1 : 0;
+    const float inv = 1.0f / l_tot;
     if (row < n_rows) {
       bf16_t* op = p.o + (int64_t)b * p.o_bs + (int64_t)tok * p.o_ts + (int64_t)head * D + 4 * h;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
-          i32x2 w = {0, 0};
-          if (inv != 0.f) {
-            w[0] = (int)pack2bf(oacc[d][4 * g4] * inv, oacc[d][4 * g4 + 1] * inv);
-            w[1] = (int)pack2bf(oacc[d][4 * g4 + 2] * inv, oacc[d][4 * g4 + 3] * inv);
-          }
+          i32x2 w;
+          w[0] = (int)pack2bf(oacc[d][4 * g4] * inv, oacc[d][4 * g4 + 1] * inv) & keep;
+          w[1] = (int)pack2bf(oacc[d][4 * g4 + 2] * inv, oacc[d][4 * g4 + 3] * inv) & keep;
           *reinterpret_cast<i32x2*>(op + 32 * d + 8 * g4) = w;
         }
     }
@@ -485,6 +536,7 @@ int fdm_attn_window(void* o, const void* q, const void* k, const void* v, const 
   if ((reinterpret_cast<uintptr_t>(q_lens) | reinterpret_cast<uintptr_t>(kv_lens)) & 3) return FDM_ERR_INVALID;
   const int64_t group = q_heads / kv_heads;
   // places, rows and items are 32-bit numbers in the kernel (addresses are 64-bit)
+  if (k_tok_stride > (1 << 22) || v_tok_stride > (1 << 22)) return FDM_ERR_UNSUPPORTED;      // (a tile's lane offsets are 32-bit)
   if (sk > (1 << 30) || sq > (1 << 30) || sq * group > (1 << 30) || batch > (1 << 24)) return FDM_ERR_UNSUPPORTED;
   const int64_t win = window < sk ? window : (sk > 0 ? sk : 1), snk = sinks < sk ? sinks : sk;      // the same keys, and no overflow
   const WindowPlan w = window_plan(batch, sq, sk, kv_heads, group, head_dim, win, snk);

@@ -467,7 +467,7 @@ int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, c
 
 /* Causal attention with a sliding window and sinks (ABI 21): prompts, chunks of a prompt behind a cache, single tokens.
  *   q [batch, sq, q_heads * head_dim], k / v [batch, sk, kv_heads * head_dim], o as q; bf16, batch and token strides in elements (multiples of 8, 16-byte
- *   aligned tensors); q_heads a multiple of kv_heads; head_dim 64 or 128.
+ *   aligned tensors; k's and v's token strides <= 2^22); q_heads a multiple of kv_heads; head_dim 64 or 128.
  *   q_lens, kv_lens: int32 [batch] on the device, or NULL for sq / sk (values outside 0 .. sq / sk count as the nearest).  The queries of a sequence are
  *   the last q_len of its kv_len tokens: row t < q_len is at place kv_len - q_len + t and sees key j iff j <= place and (place - j < window or j < sinks).
  *   Rows at or past q_len, and rows that see nothing, are zeros.  Keys at or past kv_len are not read; what a row does not see does not reach it, NaNs
