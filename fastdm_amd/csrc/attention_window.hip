@@ -36,14 +36,15 @@ struct WindowParams {
   int window, sinks;
   int n_blocks;         // row blocks of a (batch, kv head)
   int parts;            // parts a block's tile list is cut into
-  int n_items, chunk;   // batch * kv_heads * n_blocks * parts; consecutive ones per XCD
+  int classes;          // of (batch, kv head) pairs, one or more XCDs each: 1, 2, 4 or 8
   float scale_log2e;
   float* ws_o;          // parts > 1: [batch * kv_heads * n_blocks][parts][rows of a block][D], unnormalised
   float* ws_ml;         // ... [..][..][rows][2]: maximum (exp2 domain), sum
 };
 
-template <int D, int WR, int WK, int KW>
-__global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_kernel(const WindowParams p) {
+// ST: tiles in the LDS ring (one being worked on, the others on their way)
+template <int D, int WR, int WK, int KW, int ST, int OCC>
+__global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const WindowParams p) {
   constexpr int NT = 64 * WR * WK, RB = 32 * WR, KT = KW * WK;
   constexpr int NKT = KW / 32;            // 32-key S^T tiles per wave and key tile
   constexpr int CPR = D / 8;              // 16-byte pieces per key
@@ -52,21 +53,23 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
   constexpr int LD = KT * CPR / NT;       // LDS-DMA pieces per thread and tile of K (and of V)
   constexpr int KSTEPS = D / 16, DT = D / 32;
   static_assert(KT * CPR % NT == 0 && LD >= 1);
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * TILE_BYTES];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[ST * 2 * TILE_BYTES];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave % WR, wk = wave / WR;
   const int lq = lane & 31, h = lane >> 5;
 
-  // consecutive items run on one XCD, whose L2 then holds the window they share
-  const int xcd = blockIdx.x & 7, seat = blockIdx.x >> 3;
-  const int item = ((seat / p.chunk) * 8 + xcd) * p.chunk + seat % p.chunk;
-  if (item >= p.n_items) return;
-  const int part = item % p.parts;
-  const int unit = item / p.parts;
-  const int rb = p.n_blocks - 1 - unit % p.n_blocks;      // long lists first
-  const int bk = unit / p.n_blocks;
+  // The blocks that run at one time on an XCD share its L2: a class of (batch, kv head) pairs belongs to 8 / classes XCDs (classes: the largest
+  // divisor of 8 that deals the pairs out evenly), and their row blocks are taken from the last, longest lists to the first, pair by pair.
+  // Against runs of consecutive row blocks per XCD: 16384 tokens, window 4096, 8 pairs 1060 -> 944 us; open window 2664 -> 1979 us.
+  const int per = p.batch * p.kv_heads / p.classes;
+  const int it = (blockIdx.x >> 3) * (8 / p.classes) + (blockIdx.x & 7) / p.classes;
+  const int part = it % p.parts;
+  const int rb = p.n_blocks - 1 - it / p.parts / per;
+  const int bk = (blockIdx.x & 7) % p.classes + p.classes * (it / p.parts % per);
+  if (rb < 0) return;
+  const int unit = bk * p.n_blocks + rb;
   const int b = bk / p.kv_heads, kvh = bk % p.kv_heads;
   const int G = p.group;
 
@@ -163,8 +166,8 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
   for (int d = 0; d < DT; ++d)
     vld[d] = TILE_BYTES + (wk * KW + 4 * h + tq) * ROWB + (uint32_t)Swz<D>::v(4 * h + tq, d * 4 + 2 * (gi & 1) + (tp >> 1)) * 16 + 8 * (tp & 1);
 
-  // key kk of a tile whose first key is `hi` in front of the row's place: 0 <= hi - kk < window, or a sink (`sink` <= hi + 1).  No branch: | and not ||
-  auto sees = [&](int hi, int sink, int kk) { return ((unsigned)(hi - kk) < (unsigned)p.window) | (kk < sink); };
+  // the n lowest bits (n < 0: none, n > 32: all)
+  auto below = [](int n) -> uint32_t { return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u; };
 
   // one key tile for this wave; base: place of its first key.  KIND 0: every row sees every key, 1: masked, 2: masked, values that are not finite apart
   auto process = [&](auto kind_c, int base, uint32_t buf) {
@@ -183,16 +186,19 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
         const i32x4 kf = *reinterpret_cast<const i32x4*>(sb + (kld0 ^ (uint32_t)(ks << 5)) + n * 32 * ROWB);
         s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[ks]), s[n], 0, 0, 0);
       }
+    uint32_t seen[NKT];                         // MASK: bit kk of seen[n]: the row sees key base + 32 n + 4 h + kk
     if constexpr (MASK) {
-      const int at = base + 4 * h;              // element e of tile n is key at + 32 n + (e & 3) + 8 (e >> 2)
-      const int hi = place - at, sink = min(p.sinks - at, hi + 1);
 #pragma unroll
-      for (int n = 0; n < NKT; ++n)
+      for (int n = 0; n < NKT; ++n) {
+        const int at = base + n * 32 + 4 * h;
+        seen[n] = (below(place - at + 1) & ~below(place - p.window - at + 1)) | (below(p.sinks - at) & below(place - at + 1));
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int kk = n * 32 + (e & 3) + 8 * (e >> 2);
-          s[n][e] = sees(hi, sink, kk) ? s[n][e] : -INFINITY;
+        for (int e = 0; e < 16; ++e) {          // one v_bfe_i32 and one v_bfi_b32
+          const int on = (int)(seen[n] << (31 - (e & 3) - 8 * (e >> 2))) >> 31;
+          const float score = s[n][e];          // (hipcc takes the bit cast of a vector element for that of element 0)
+          s[n][e] = __builtin_bit_cast(float, (__builtin_bit_cast(int, score) & on) | (~on & (int)0xff800000));
         }
+      }
     }
     // row maximum: med3(a, b, +inf) is max without the canonicalisation hipcc puts in front of fmaxf
     float mx = s[0][0];
@@ -237,11 +243,10 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
       for (int u = 0; u < 2; ++u) {
         i32x4 see;                              // KIND 2: 1.0 where the row sees the key, laid out as P
         if constexpr (KIND == 2) {
-          const int hi = place - base - 4 * h, sink = min(p.sinks - base - 4 * h, hi + 1);
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const int k0 = n * 32 + 16 * u + 8 * (w >> 1) + 2 * (w & 1);
-            see[w] = (sees(hi, sink, k0) ? 0x3f80 : 0) | (sees(hi, sink, k0 + 1) ? 0x3f800000 : 0);
+            const int k0 = 16 * u + 8 * (w >> 1) + 2 * (w & 1);
+            see[w] = ((seen[n] >> k0 & 1) ? 0x3f80 : 0) | ((seen[n] >> (k0 + 1) & 1) ? 0x3f800000 : 0);
           }
         }
 #pragma unroll
@@ -297,22 +302,34 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
     }
   };
   int buf = 0, i = i_begin;
-  auto arrive = [&](bool masked) {                      // tile i is there, tile i + 1 on its way
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // this wave's pieces of tile i have landed ...
-    if (masked) clean(tile_at(i) * KT, buf);
-    __syncthreads();                                    // ... and everybody's; the other buffer has been read
-    if (i + 1 < i_end) stage(tile_at(i + 1), buf ^ 1);
+  auto fill = [&]() {
+#pragma unroll
+    for (int j = 0; j < ST - 1; ++j)
+      if (i_begin + j < i_end) stage(tile_at(i_begin + j), j);
   };
-  if (i_begin < i_end) stage(tile_at(i_begin), 0);
+  auto arrive = [&](bool masked) {                      // tile i is there, the ST - 1 tiles behind it on their way
+    if (ST > 2 && i + ST - 2 < i_end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 2) * 2 * LD) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this wave's pieces of tile i have landed ...
+    if (masked) clean(tile_at(i) * KT, buf);
+    __syncthreads();                                    // ... and everybody's; the slot of tile i - 1 has been read
+    if (i + ST - 1 < i_end) stage(tile_at(i + ST - 1), buf == 0 ? ST - 1 : buf - 1);
+  };
+  auto on = [&]() {
+    ++i;
+    buf = buf == ST - 1 ? 0 : buf + 1;
+  };
+  fill();
+#pragma unroll
+  for (int ks = 0; ks < KSTEPS; ++ks) asm volatile("" ::"v"(qf[ks]));      // (there before the loop: its waits count DMAs alone)
   for (int stretch = 0; stretch < 3; ++stretch) {
     const int to = min(stretch == 0 ? mid_lo : stretch == 1 ? mid_hi : n_list, i_end);
     if (stretch == 1) {
-      for (; i < to; ++i, buf ^= 1) {
+      for (; i < to; on()) {
         arrive(false);
         if (has_rows) process(std::integral_constant<int, 0>{}, 0, buf * 2 * TILE_BYTES);
       }
     } else {
-      for (; i < to; ++i, buf ^= 1) {
+      for (; i < to; on()) {
         arrive(true);
         const int base = tile_at(i) * KT + wk * KW;
         if (has_rows && base <= wp_hi && (base + KW > wp_lo - p.window + 1 || base < p.sinks)) process(std::integral_constant<int, 1>{}, base, buf * 2 * TILE_BYTES);
@@ -328,8 +345,8 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
     l_run = 0.f;
     buf = 0;
     i = i_begin;
-    if (i_begin < i_end) stage(tile_at(i_begin), 0);
-    for (; i < i_end; ++i, buf ^= 1) {
+    fill();
+    for (; i < i_end; on()) {
       arrive(true);
       const int base = tile_at(i) * KT + wk * KW;
       if (has_rows && base <= wp_hi && (base + KW > wp_lo - p.window + 1 || base < p.sinks)) process(std::integral_constant<int, 2>{}, base, buf * 2 * TILE_BYTES);
@@ -337,100 +354,69 @@ __global__ void __launch_bounds__(64 * WR * WK, WK == 1 ? 2 : 1) attn_window_ker
   }
 
   float l_tot = l_run + __shfl_xor(l_run, 32, 64);
-  const int64_t unit_part = (int64_t)unit * p.parts + part;
-  if constexpr (WK == 1) {
-    if (p.parts > 1) {
-      float* wo = p.ws_o + (unit_part * RB + wr * 32 + lq) * D + 4 * h;
+  if constexpr (WK > 1) {
+    // ---- the key waves' shares are merged through LDS by the first of them, register by register (the same rows lie in the same lanes)
+    constexpr int R4 = DT * 4;                            // f32x4 per lane
+    static_assert((WK - 1) * WR * 64 * (R4 * 16 + 8) <= ST * 2 * TILE_BYTES);
+    f32x4* so = reinterpret_cast<f32x4*>(smem);
+    float* sml = reinterpret_cast<float*>(smem + (WK - 1) * WR * R4 * 1024);
+    __syncthreads();                                      // the last tile has been read
+    if (wk > 0) {
+      const int w = (wk - 1) * WR + wr;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4)
-          *reinterpret_cast<f32x4*>(wo + 32 * d + 8 * g4) = f32x4{oacc[d][4 * g4], oacc[d][4 * g4 + 1], oacc[d][4 * g4 + 2], oacc[d][4 * g4 + 3]};
-      if (h == 0) {
-        float* ml = p.ws_ml + (unit_part * RB + wr * 32 + lq) * 2;
-        ml[0] = m_run;
-        ml[1] = l_tot;
-      }
-      return;
+          so[(w * R4 + d * 4 + g4) * 64 + lane] = f32x4{oacc[d][4 * g4], oacc[d][4 * g4 + 1], oacc[d][4 * g4 + 2], oacc[d][4 * g4 + 3]};
+      sml[w * 128 + lane] = m_run;
+      sml[w * 128 + 64 + lane] = l_tot;
     }
-    const int keep = live && l_tot != 0.f ? -1 : 0;
-    const float inv = 1.0f / l_tot;
-    if (row < n_rows) {
-      bf16_t* op = p.o + (int64_t)b * p.o_bs + (int64_t)tok * p.o_ts + (int64_t)head * D + 4 * h;
+    __syncthreads();
+    if (wk > 0) return;
+#pragma unroll
+    for (int k2 = 1; k2 < WK; ++k2) {
+      const int w = (k2 - 1) * WR + wr;
+      const float m2 = sml[w * 128 + lane], m_new = fmaxf(m_run, m2);
+      const float a1 = __builtin_amdgcn_exp2f(m_run - m_new), a2 = __builtin_amdgcn_exp2f(m2 - m_new);
+      m_run = m_new;
+      l_tot = l_tot * a1 + sml[w * 128 + 64 + lane] * a2;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
-          i32x2 w;
-          w[0] = (int)pack2bf(oacc[d][4 * g4] * inv, oacc[d][4 * g4 + 1] * inv) & keep;
-          w[1] = (int)pack2bf(oacc[d][4 * g4 + 2] * inv, oacc[d][4 * g4 + 3] * inv) & keep;
-          *reinterpret_cast<i32x2*>(op + 32 * d + 8 * g4) = w;
+          const f32x4 x = so[(w * R4 + d * 4 + g4) * 64 + lane];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) oacc[d][4 * g4 + c] = oacc[d][4 * g4 + c] * a1 + x[c] * a2;
         }
     }
-  } else {
-    // ---- the waves' shares of the keys are merged through LDS: [wave][row][D + 4], the padding keeps rows off each other's banks
-    static_assert(WR == 1);
-    constexpr int LROW = D + 4;
-    static_assert(WK * 32 * (LROW + 2) * 4 <= 4 * TILE_BYTES);
-    float* lo = reinterpret_cast<float*>(smem);
-    float* lml = lo + WK * 32 * LROW;
-    __syncthreads();                                    // the last tile has been read
-    float* mine = lo + (wk * 32 + lq) * LROW + 4 * h;
+  }
+  if (row >= n_rows) return;
+  if (p.parts > 1) {
+    const int64_t at = ((int64_t)unit * p.parts + part) * RB + wr * 32 + lq;
+    float* wo = p.ws_o + at * D + 4 * h;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4)
-        *reinterpret_cast<f32x4*>(mine + 32 * d + 8 * g4) = f32x4{oacc[d][4 * g4], oacc[d][4 * g4 + 1], oacc[d][4 * g4 + 2], oacc[d][4 * g4 + 3]};
+        *reinterpret_cast<f32x4*>(wo + 32 * d + 8 * g4) = f32x4{oacc[d][4 * g4], oacc[d][4 * g4 + 1], oacc[d][4 * g4 + 2], oacc[d][4 * g4 + 3]};
     if (h == 0) {
-      lml[(wk * 32 + lq) * 2] = m_run;
-      lml[(wk * 32 + lq) * 2 + 1] = l_tot;
+      p.ws_ml[at * 2] = m_run;
+      p.ws_ml[at * 2 + 1] = l_tot;
     }
-    __syncthreads();
-    constexpr int TPR = NT / 32, PER = D / TPR;         // threads per row, values each
-    static_assert(PER % 4 == 0);
-    const int r = tid / TPR, d0 = (tid % TPR) * PER;
-    float m = -3.0e38f, l = 0.f, f[WK];
-#pragma unroll
-    for (int w = 0; w < WK; ++w) m = fmaxf(m, lml[(w * 32 + r) * 2]);
-#pragma unroll
-    for (int w = 0; w < WK; ++w) {
-      f[w] = __builtin_amdgcn_exp2f(lml[(w * 32 + r) * 2] - m);
-      l += f[w] * lml[(w * 32 + r) * 2 + 1];
-    }
-    float acc[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) acc[j] = 0.f;
-#pragma unroll
-    for (int w = 0; w < WK; ++w)
-#pragma unroll
-      for (int j = 0; j < PER; j += 4) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(lo + (w * 32 + r) * LROW + d0 + j);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[j + c] += f[w] * x[c];
-      }
-    const int grow = rb * RB + r;
-    if (grow >= n_rows) return;
-    if (p.parts > 1) {
-      float* wo = p.ws_o + (unit_part * RB + r) * D + d0;
-#pragma unroll
-      for (int j = 0; j < PER; j += 4) *reinterpret_cast<f32x4*>(wo + j) = f32x4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]};
-      if (d0 == 0) {
-        p.ws_ml[(unit_part * RB + r) * 2] = m;
-        p.ws_ml[(unit_part * RB + r) * 2 + 1] = l;
-      }
-      return;
-    }
-    const int t = grow / G;
-    const bool ok = t < q_len && l != 0.f;
-    const float inv = ok ? 1.0f / l : 0.f;
-    bf16_t* op = p.o + (int64_t)b * p.o_bs + (int64_t)t * p.o_ts + (int64_t)(kvh * G + grow % G) * D + d0;
-#pragma unroll
-    for (int j = 0; j < PER; j += 4) {
-      i32x2 w = {0, 0};
-      if (ok) w = i32x2{(int)pack2bf(acc[j] * inv, acc[j + 1] * inv), (int)pack2bf(acc[j + 2] * inv, acc[j + 3] * inv)};
-      *reinterpret_cast<i32x2*>(op + j) = w;
-    }
+    return;
   }
+  const int keep = live && l_tot != 0.f ? -1 : 0;
+  const float inv = 1.0f / l_tot;
+  bf16_t* op = p.o + (int64_t)b * p.o_bs + (int64_t)tok * p.o_ts + (int64_t)head * D + 4 * h;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      i32x2 w;
+      w[0] = (int)pack2bf(oacc[d][4 * g4] * inv, oacc[d][4 * g4 + 1] * inv) & keep;
+      w[1] = (int)pack2bf(oacc[d][4 * g4 + 2] * inv, oacc[d][4 * g4 + 3] * inv) & keep;
+      *reinterpret_cast<i32x2*>(op + 32 * d + 8 * g4) = w;
+    }
 }
 
 // ---- merge of the parts: one row per D / 4 threads, o = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i in the parts' order
@@ -442,7 +428,7 @@ __global__ void __launch_bounds__(256) attn_window_merge_kernel(const WindowPara
   if (idx >= n_rows * p.batch * p.kv_heads) return;
   const int64_t bk = idx / n_rows, row = idx % n_rows;
   const int rb = (int)(row / rb_rows), r = (int)(row % rb_rows);
-  const int64_t unit = bk * p.n_blocks + (p.n_blocks - 1 - rb);
+  const int64_t unit = bk * p.n_blocks + rb;
   const int d0 = (threadIdx.x % TPR) * 4;
   const int b = (int)(bk / p.kv_heads), kvh = (int)(bk % p.kv_heads);
   const int tok = (int)(row / p.group), head = kvh * p.group + (int)(row % p.group);
@@ -469,28 +455,30 @@ __global__ void __launch_bounds__(256) attn_window_merge_kernel(const WindowPara
 
 // ---- host side: which form, and into how many parts
 struct WindowPlan {
-  bool few;             // single tokens and the like: WR = 1
+  int form;             // 0: one row wave, four key waves (single tokens and the like); 1: four row waves; 2: four row waves, two key waves
   int rb_rows, kt;
   int64_t n_blocks, units;
   int parts;
 };
 static WindowPlan window_plan(int64_t batch, int64_t sq, int64_t sk, int64_t kv_heads, int64_t group, int head_dim, int64_t window, int64_t sinks) {
   WindowPlan w{};
-  w.few = sq * group <= 32;
-  w.rb_rows = w.few ? 32 : 128;
-  w.kt = w.few ? (head_dim == 128 ? 128 : 256) : 64;
-  w.n_blocks = (sq * group + w.rb_rows - 1) / w.rb_rows;
+  const int64_t rows = sq * group, cus = device_cu_count();
+  const bool few = rows <= 32;
+  w.rb_rows = few ? 32 : 128;
+  w.n_blocks = (rows + w.rb_rows - 1) / w.rb_rows;
   w.units = batch * kv_heads * w.n_blocks;
+  w.form = few ? 0 : w.units > cus ? 1 : 2;
+  w.kt = w.form == 0 ? (head_dim == 128 ? 128 : 256) : w.form == 1 ? 64 : 128;
   // tiles a block walks at most, whatever the lengths on the device say
   const int64_t span = w.rb_rows / group + 1 + window;
   int64_t tiles = (span + w.kt - 1) / w.kt + 1 + (sinks + w.kt - 1) / w.kt;
   const int64_t every = (sk + w.kt - 1) / w.kt;
   if (tiles > every) tiles = every;
-  const int64_t slots = (int64_t)device_cu_count() * (w.few ? 1 : 2);
+  const int64_t slots = cus * (w.form == 1 ? 2 : 1);
   int64_t parts = 1;
   if (w.units < slots) {
     parts = slots / w.units;
-    const int64_t most = tiles / 2;
+    const int64_t most = tiles / 4;
     if (parts > most) parts = most;
     if (parts > 64) parts = 64;
     if (parts < 1) parts = 1;
@@ -499,11 +487,11 @@ static WindowPlan window_plan(int64_t batch, int64_t sq, int64_t sk, int64_t kv_
   return w;
 }
 
-template <int D, int WR, int WK, int KW>
+template <int D, int WR, int WK, int KW, int ST, int OCC>
 static int launch_window(const WindowParams& p, hipStream_t s) {
-  const int64_t per = (int64_t)8 * p.chunk;
-  const int64_t grid = (p.n_items + per - 1) / per * per;
-  attn_window_kernel<D, WR, WK, KW><<<dim3((unsigned)grid), dim3(64 * WR * WK), 0, s>>>(p);
+  const int64_t per_class = (int64_t)p.batch * p.kv_heads / p.classes * p.n_blocks * p.parts, xcds = 8 / p.classes;
+  const int64_t grid = (per_class + xcds - 1) / xcds * 8;
+  attn_window_kernel<D, WR, WK, KW, ST, OCC><<<dim3((unsigned)grid), dim3(64 * WR * WK), 0, s>>>(p);
   FDM_CHECK_LAUNCH();
   return FDM_OK;
 }
@@ -549,16 +537,18 @@ int fdm_attn_window(void* o, const void* q, const void* k, const void* v, const 
   p.q_bs = q_batch_stride; p.q_ts = q_tok_stride; p.k_bs = k_batch_stride; p.k_ts = k_tok_stride; p.v_bs = v_batch_stride; p.v_ts = v_tok_stride;
   p.o_bs = o_batch_stride; p.o_ts = o_tok_stride;
   p.batch = (int)batch; p.sq = (int)sq; p.sk = (int)sk; p.kv_heads = kv_heads; p.group = (int)group;
-  p.window = (int)win; p.sinks = (int)snk; p.n_blocks = (int)w.n_blocks; p.parts = w.parts; p.n_items = (int)items;
-  const int64_t each = (items + 7) / 8;
-  p.chunk = (int)(each < 32 ? each : 32);
+  p.window = (int)win; p.sinks = (int)snk; p.n_blocks = (int)w.n_blocks; p.parts = w.parts;
+  const int64_t pairs = batch * kv_heads;
+  p.classes = pairs % 8 == 0 ? 8 : pairs % 4 == 0 ? 4 : pairs % 2 == 0 ? 2 : 1;
   p.scale_log2e = scale * 1.4426950408889634f;
   p.ws_o = (float*)workspace;
   p.ws_ml = p.ws_o + w.units * w.parts * w.rb_rows * head_dim;
   hipStream_t s = to_stream(stream);
   int rc;
-  if (head_dim == 128) rc = w.few ? launch_window<128, 1, 4, 32>(p, s) : launch_window<128, 4, 1, 64>(p, s);
-  else rc = w.few ? launch_window<64, 1, 4, 64>(p, s) : launch_window<64, 4, 1, 64>(p, s);
+  if (head_dim == 128)
+    rc = w.form == 0 ? launch_window<128, 1, 4, 32, 2, 1>(p, s) : w.form == 1 ? launch_window<128, 4, 1, 64, 2, 2>(p, s) : launch_window<128, 4, 2, 64, 2, 2>(p, s);
+  else
+    rc = w.form == 0 ? launch_window<64, 1, 4, 64, 2, 1>(p, s) : w.form == 1 ? launch_window<64, 4, 1, 64, 2, 3>(p, s) : launch_window<64, 4, 2, 64, 2, 2>(p, s);
   if (rc != FDM_OK || w.parts == 1) return rc;
   const int64_t rows = batch * kv_heads * sq * group;
   const int per_block = 256 / (head_dim / 4);
