@@ -12,9 +12,8 @@
 //             row-major tile through ds_read_b64_tr_b16.  P is rounded to bf16 (2^-9 of each weight, averaged over the keys; the row sums are those of
 //             the unrounded weights in fp32): the matrix core's operand type.
 //   softmax   one pass, running maximum and sum in fp32, exp2 domain, O and l rescaled only where a row's maximum grew by more than 2^8.
-//   waves     WR waves over rows (32 each) times WK waves over the keys of a tile: prompts WK = 1; few rows (single tokens) WR = 1, WK = 4, merged
-//             through LDS at the end.  Where the blocks would not fill the chip, a block's tile list is cut into parts that run side by side and
-//             are merged by a second small launch.
+//   waves     WR waves over rows (32 each) times WK waves over the keys of a tile, merged through LDS at the end (window_plan says which).  Where the blocks
+//             would not fill the chip, a block's tile list is cut into parts that run side by side and are merged by a second small launch.
 //   NaN       what a row does not see does not reach it, though 0 * NaN is NaN in the matrix core: masked scores are replaced, keys past kv_len are never
 //             read, values that no row of the block sees are zeroed in LDS, and a block that finds one that is not finite among those that only some
 //             rows see starts over: product with the finite values, and a second product of marks for the rows that see one that is not.
@@ -419,69 +418,110 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
     }
 }
 
-// ---- merge of the parts: one row per D / 4 threads, o = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i in the parts' order
-template <int D>
+// ---- merge of the parts: o = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i.  D / 4 threads per row and part group; PG groups take the parts in turn (long
+//      lists of parts are a chain of loads otherwise) and are joined through LDS, all in a fixed order.
+template <int D, int PG>
 __global__ void __launch_bounds__(256) attn_window_merge_kernel(const WindowParams p, int rb_rows) {
-  constexpr int TPR = D / 4;
+  constexpr int TPR = D / 4, ROWS = 256 / (TPR * PG);
   const int64_t n_rows = (int64_t)p.sq * p.group;
-  const int64_t idx = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-  if (idx >= n_rows * p.batch * p.kv_heads) return;
-  const int64_t bk = idx / n_rows, row = idx % n_rows;
-  const int rb = (int)(row / rb_rows), r = (int)(row % rb_rows);
-  const int64_t unit = bk * p.n_blocks + rb;
-  const int d0 = (threadIdx.x % TPR) * 4;
+  const int pg = threadIdx.x / TPR % PG, lane = threadIdx.x % TPR, r_blk = threadIdx.x / (TPR * PG);
+  const int64_t idx = (int64_t)blockIdx.x * ROWS + r_blk;
+  const bool there = idx < n_rows * p.batch * p.kv_heads;
+  const int64_t bk = there ? idx / n_rows : 0, row = there ? idx % n_rows : 0;
+  const int64_t unit = bk * p.n_blocks + row / rb_rows;
+  const int64_t first = unit * p.parts * rb_rows + row % rb_rows;       // part i's row: + i * rb_rows
+  float m = -3.0e38f, l = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = pg; i < p.parts; i += PG) {
+    const int64_t at = first + (int64_t)i * rb_rows;
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p.ws_o + at * D + lane * 4);
+    const float m2 = p.ws_ml[at * 2], l2 = p.ws_ml[at * 2 + 1];
+    const float m_new = fmaxf(m, m2), a1 = __builtin_amdgcn_exp2f(m - m_new), a2 = __builtin_amdgcn_exp2f(m2 - m_new);
+    m = m_new;
+    l = l * a1 + l2 * a2;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] = acc[c] * a1 + x[c] * a2;
+  }
+  if constexpr (PG > 1) {
+    __shared__ f32x4 so[256];
+    __shared__ float sm[256], sl[256];
+    so[threadIdx.x] = acc;
+    sm[threadIdx.x] = m;
+    sl[threadIdx.x] = l;
+    __syncthreads();
+    if (pg > 0) return;
+#pragma unroll
+    for (int g = 1; g < PG; ++g) {
+      const int t = threadIdx.x + g * TPR;
+      const f32x4 x = so[t];
+      const float m_new = fmaxf(m, sm[t]), a1 = __builtin_amdgcn_exp2f(m - m_new), a2 = __builtin_amdgcn_exp2f(sm[t] - m_new);
+      m = m_new;
+      l = l * a1 + sl[t] * a2;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[c] = acc[c] * a1 + x[c] * a2;
+    }
+  }
+  if (!there) return;
   const int b = (int)(bk / p.kv_heads), kvh = (int)(bk % p.kv_heads);
   const int tok = (int)(row / p.group), head = kvh * p.group + (int)(row % p.group);
   int q_len = p.sq;
   if (p.q_lens != nullptr) q_len = min(max(p.q_lens[b], 0), p.sq);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float m = -3.0e38f, l = 0.f;
-  for (int i = 0; i < p.parts; ++i) m = fmaxf(m, p.ws_ml[((unit * p.parts + i) * rb_rows + r) * 2]);
-  for (int i = 0; i < p.parts; ++i) {
-    const int64_t at = (unit * p.parts + i) * rb_rows + r;
-    const float f = __builtin_amdgcn_exp2f(p.ws_ml[at * 2] - m);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p.ws_o + at * D + d0);
-    l += f * p.ws_ml[at * 2 + 1];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) acc[c] += f * x[c];
+  const int keep = tok < q_len && l != 0.f ? -1 : 0;
+  const float inv = 1.0f / l;
+  const i32x2 w = {(int)pack2bf(acc[0] * inv, acc[1] * inv) & keep, (int)pack2bf(acc[2] * inv, acc[3] * inv) & keep};
+  *reinterpret_cast<i32x2*>(p.o + (int64_t)b * p.o_bs + (int64_t)tok * p.o_ts + (int64_t)head * D + lane * 4) = w;
+}
+
+template <int D>
+static int launch_merge(const WindowParams& p, int rb_rows, hipStream_t s) {
+  const int64_t rows = (int64_t)p.batch * p.kv_heads * p.sq * p.group;
+  if (p.parts > 4) {
+    constexpr int PG = 256 / (D / 4);
+    attn_window_merge_kernel<D, PG><<<dim3((unsigned)rows), dim3(256), 0, s>>>(p, rb_rows);
+  } else {
+    constexpr int per = 256 / (D / 4);
+    attn_window_merge_kernel<D, 1><<<dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s>>>(p, rb_rows);
   }
-  i32x2 w = {0, 0};
-  if (tok < q_len && l != 0.f) {
-    const float inv = 1.0f / l;
-    w = i32x2{(int)pack2bf(acc[0] * inv, acc[1] * inv), (int)pack2bf(acc[2] * inv, acc[3] * inv)};
-  }
-  *reinterpret_cast<i32x2*>(p.o + (int64_t)b * p.o_bs + (int64_t)tok * p.o_ts + (int64_t)head * D + d0) = w;
+  FDM_CHECK_LAUNCH();
+  return FDM_OK;
 }
 
 // ---- host side: which form, and into how many parts
+//   0  up to 32 rows (single tokens and the like), 32-key tiles: blocks of one wave, no barrier to wait at, four (head_dim 64: eight) of them on a CU, each
+//      with its own share of the list.  Four waves on a 128-key tile instead: 128 sequences of 512 keys, 32/8 heads x 128: 42 -> 59 us; one sequence,
+//      window 4096: 11 -> 15 us.
+//   1  the chip full of 128-row blocks: four row waves, 64-key tiles, two (head_dim 64: three) blocks on a CU whose phases drift apart, so that one's
+//      softmax runs under the other's products.  64-row blocks read each tile twice as often: 16384 tokens, window 4096: 1055 -> 1593 us.
+//   2  up to one 128-row block per CU: 64-row blocks of two row waves x two key waves, two of them on a CU.  Against form 3: 600 tokens, 24 heads x 64:
+//      12.1 -> 9.7 us, x 128: 17.2 -> 13.5 us; 1200 tokens, 24 x 128: 26.6 -> 24.5 us.
+//   3  the same with long lists (2048 keys and more, head_dim 128): 128-row blocks, four row waves x two key waves, half the reads of form 2.  Against
+//      form 2: 8 sequences of 64 tokens, window 4096: 60.2 -> 53.4 us; 512-token chunks of 2, window 2048: 47.7 -> 46.0 us.
 struct WindowPlan {
-  int form;             // 0: one row wave, four key waves (single tokens and the like); 1: four row waves; 2: four row waves, two key waves
-  int rb_rows, kt;
+  int form, rb_rows, kt;
   int64_t n_blocks, units;
   int parts;
 };
 static WindowPlan window_plan(int64_t batch, int64_t sq, int64_t sk, int64_t kv_heads, int64_t group, int head_dim, int64_t window, int64_t sinks) {
   WindowPlan w{};
   const int64_t rows = sq * group, cus = device_cu_count();
-  const bool few = rows <= 32;
-  w.rb_rows = few ? 32 : 128;
+  int64_t keys = 128 / group + 1 + window + sinks;       // that the lists of 128 rows hold at most, whatever the lengths on the device say
+  if (keys > sk) keys = sk;
+  w.form = rows <= 32 ? 0 : batch * kv_heads * ((rows + 127) / 128) > cus ? 1 : head_dim == 128 && keys >= 2048 ? 3 : 2;
+  w.rb_rows = w.form == 0 ? 32 : w.form == 2 ? 64 : 128;
+  w.kt = w.form == 0 ? 32 : w.form == 3 ? 128 : w.form == 1 || head_dim == 128 ? 64 : 128;
   w.n_blocks = (rows + w.rb_rows - 1) / w.rb_rows;
   w.units = batch * kv_heads * w.n_blocks;
-  w.form = few ? 0 : w.units > cus ? 1 : 2;
-  w.kt = w.form == 0 ? (head_dim == 128 ? 128 : 256) : w.form == 1 ? 64 : 128;
-  // tiles a block walks at most, whatever the lengths on the device say
-  const int64_t span = w.rb_rows / group + 1 + window;
-  int64_t tiles = (span + w.kt - 1) / w.kt + 1 + (sinks + w.kt - 1) / w.kt;
-  const int64_t every = (sk + w.kt - 1) / w.kt;
-  if (tiles > every) tiles = every;
-  const int64_t slots = cus * (w.form == 1 ? 2 : 1);
+  // where the blocks leave places on the chip free: parts of at least two (form 0) or four tiles; not for lists under 16 tiles, the merge is a launch of
+  // its own (one token, window 128: 8.1 us in one part, 7.3 in two, but 5 us more on the host)
+  const int64_t slots = cus * (w.form == 0 ? (head_dim == 128 ? 4 : 8) : w.form == 3 ? 1 : 2);
+  const int64_t tiles = (keys + w.kt - 1) / w.kt;
   int64_t parts = 1;
-  if (w.units < slots) {
+  if (w.units < slots && tiles >= 16) {
     parts = slots / w.units;
-    const int64_t most = tiles / 4;
+    const int64_t most = tiles / (w.form == 0 ? 2 : 4);
     if (parts > most) parts = most;
     if (parts > 64) parts = 64;
-    if (parts < 1) parts = 1;
   }
   w.parts = (int)parts;
   return w;
@@ -546,17 +586,11 @@ int fdm_attn_window(void* o, const void* q, const void* k, const void* v, const 
   hipStream_t s = to_stream(stream);
   int rc;
   if (head_dim == 128)
-    rc = w.form == 0 ? launch_window<128, 1, 4, 32, 2, 1>(p, s) : w.form == 1 ? launch_window<128, 4, 1, 64, 2, 2>(p, s) : launch_window<128, 4, 2, 64, 2, 2>(p, s);
+    rc = w.form == 0 ? launch_window<128, 1, 1, 32, 2, 1>(p, s) : w.form == 1 ? launch_window<128, 4, 1, 64, 2, 2>(p, s) : w.form == 2 ? launch_window<128, 2, 2, 32, 2, 2>(p, s) : launch_window<128, 4, 2, 64, 2, 2>(p, s);
   else
-    rc = w.form == 0 ? launch_window<64, 1, 4, 64, 2, 1>(p, s) : w.form == 1 ? launch_window<64, 4, 1, 64, 2, 3>(p, s) : launch_window<64, 4, 2, 64, 2, 2>(p, s);
+    rc = w.form == 0 ? launch_window<64, 1, 1, 32, 2, 2>(p, s) : w.form == 1 ? launch_window<64, 4, 1, 64, 2, 3>(p, s) : launch_window<64, 2, 2, 64, 2, 2>(p, s);
   if (rc != FDM_OK || w.parts == 1) return rc;
-  const int64_t rows = batch * kv_heads * sq * group;
-  const int per_block = 256 / (head_dim / 4);
-  const unsigned grid = (unsigned)((rows + per_block - 1) / per_block);
-  if (head_dim == 128) attn_window_merge_kernel<128><<<dim3(grid), dim3(256), 0, s>>>(p, w.rb_rows);
-  else attn_window_merge_kernel<64><<<dim3(grid), dim3(256), 0, s>>>(p, w.rb_rows);
-  FDM_CHECK_LAUNCH();
-  return FDM_OK;
+  return head_dim == 128 ? launch_merge<128>(p, w.rb_rows, s) : launch_merge<64>(p, w.rb_rows, s);
 }
 
 }  // extern "C"
