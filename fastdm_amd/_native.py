@@ -291,50 +291,52 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def need_gpu(what, *tensors):
-    """Every tensor on one GPU, and none that autograd would expect a gradient through (the operators have no backward)."""
-    import torch
-    dev = None
+def gpu_of(what, *tensors):
+    """Index of the GPU that holds every one of `tensors` (None entries are skipped); none may be one that autograd expects a gradient through (the
+    operators have no backward).  The first one is always there."""
+    index = tensors[0].get_device()
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise RuntimeError(f"{what}: fastdm_amd operators need GPU tensors (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"{what}: tensors on {dev} and {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{what}: forward only -- call it under torch.no_grad() or with tensors that require no gradient")
+        if t.get_device() != index or index < 0:
+            if index < 0 or not t.is_cuda:
+                raise RuntimeError(f"{what}: fastdm_amd operators need GPU tensors (no CPU fallback)")
+            raise RuntimeError(f"{what}: tensors on GPU {index} and {t.get_device()}")
+        if t.requires_grad:
+            import torch
+            if torch.is_grad_enabled():
+                raise RuntimeError(f"{what}: forward only -- call it under torch.no_grad() or with tensors that require no gradient")
+    return index
+
+
+def launch(what, index, fn, *args):
+    """fn(*args, stream) on GPU `index`: its current stream, and itself as the current device while the kernel is launched."""
+    if index == _current_device():
+        rc = fn(*args, stream(index))
+    else:
+        import torch
+        with torch.cuda.device(index):
+            rc = fn(*args, stream(index))
+    if rc != 0:
+        check(rc, what)
+
+
+def _current_device():
+    global _current_device
+    import torch
+    _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device      # (the call behind torch.cuda.current_device)
+    return _current_device()
 
 
 def row_stride(t, what):
     """Row stride of a [rows, width] matrix whose rows may be slices of wider ones (one row: any)."""
     rows, width = t.shape
-    assert t.stride(1) == 1 or width == 1, f"{what}: rows must be dense"
+    stride, unit = t.stride()
+    assert unit == 1 or width == 1, f"{what}: rows must be dense"
     if rows <= 1:
         return width
-    assert t.stride(0) >= width, f"{what}: rows overlap"
-    return t.stride(0)
-
-
-class _Here:
-    """The tensors' device is the current one already: nothing to switch."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_here = _Here()
-
-
-def on_device(t):
-    """Context in which a launch goes to `t`'s device (a kernel launched on another device's stream is an error)."""
-    import torch
-    return _here if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    assert stride >= width, f"{what}: rows overlap"
+    return stride
 
 
 _raw_stream = None

@@ -216,20 +216,60 @@ struct RopeAtArgs {
   int per_head;           // ... per head
   int n_turn;             // ... of these: rotated ones (the others are copied)
   int tok_per_block;
+  uint32_t items_magic, head_magic;      // ceil(2^32 / items), ceil(2^32 / per_head); 0 for 1
   float amplitude;
 };
 
 constexpr int ROPE_MAX_HALF = 128, ROPE_MAX_TOK = 16;
 
-// V: elements per vector.  Half layout: an item is V low and V high elements; interleaved: V elements (V / 2 pairs).
+// V: elements per vector.  An item is, rotated: V low and V high elements (half layout) or V elements (interleaved: V / 2 pairs; V == 1: one pair, element by
+// element); behind the rotated part: V elements copied as they are.
+template <int V, bool NEOX>
+struct RopeItem {
+  static constexpr int W = !NEOX && V == 1 ? 2 : V;
+  typedef uint16_t vec_t __attribute__((ext_vector_type(V == 1 ? 2 : V)));
+  uint16_t a[W], b[W];
+
+  static __device__ __forceinline__ void get(uint16_t (&x)[W], const bf16_t* p, int n) {
+    if constexpr (V == 1) {
+      x[0] = p[0];
+      if (W == 2 && n == 2) x[W - 1] = p[1];
+    } else {
+      const vec_t v = *reinterpret_cast<const vec_t*>(p);
+#pragma unroll
+      for (int j = 0; j < W; ++j) x[j] = v[j];
+    }
+  }
+  static __device__ __forceinline__ void put(bf16_t* p, const uint16_t (&x)[W], int n) {
+    if constexpr (V == 1) {
+      p[0] = x[0];
+      if (W == 2 && n == 2) p[1] = x[W - 1];
+    } else {
+      vec_t v;
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[j] = x[j];
+      *reinterpret_cast<vec_t*>(p) = v;
+    }
+  }
+};
+
 template <int V, bool NEOX>
 __global__ void __launch_bounds__(256) rope_at_kernel(const RopeAtArgs p) {
-  typedef uint16_t vec_t __attribute__((ext_vector_type(V == 1 ? 2 : V)));
-  extern __shared__ float2 turn_cs[];      // [tok_per_block][rot / 2]
+  typedef RopeItem<V, NEOX> Item;
+  constexpr int U = 4;                           // items per thread and turn: their loads go out together
+  extern __shared__ float2 turn_cs[];            // [tok_per_block][rot / 2]
+  __shared__ int64_t at_q[ROPE_MAX_TOK], at_k[ROPE_MAX_TOK], at_qo[ROPE_MAX_TOK], at_ko[ROPE_MAX_TOK];
   const int half = p.rot >> 1;
   const int64_t tok0 = (int64_t)blockIdx.x * p.tok_per_block;
   const int ntok = (int)min((int64_t)p.tok_per_block, p.tokens - tok0);
 
+  if (threadIdx.x < ntok) {
+    const int64_t tok = tok0 + threadIdx.x, b = tok / p.seq, s = tok - b * p.seq;
+    at_q[threadIdx.x] = b * p.q_bs + s * p.q_ts;
+    at_k[threadIdx.x] = b * p.k_bs + s * p.k_ts;
+    at_qo[threadIdx.x] = b * p.qo_bs + s * p.qo_ts;
+    at_ko[threadIdx.x] = b * p.ko_bs + s * p.ko_ts;
+  }
   for (int i = threadIdx.x; i < ntok * half; i += 256) {
     const int t = i / half, f = i - t * half;
     const int64_t tok = tok0 + t;
@@ -247,75 +287,55 @@ __global__ void __launch_bounds__(256) rope_at_kernel(const RopeAtArgs p) {
   }
   __syncthreads();
 
+  auto by = [](int i, uint32_t magic) { return magic ? (int)__umulhi((uint32_t)i, magic) : i; };
   const int total = ntok * p.items;
-  for (int i = threadIdx.x; i < total; i += 256) {
-    const int t = i / p.items;
-    int it = i - t * p.items;
-    const int64_t tok = tok0 + t;
-    const int64_t b = tok / p.seq, s = tok - b * p.seq;
-    int hd = it / p.per_head;
-    it -= hd * p.per_head;
-    const bf16_t* src;
-    bf16_t* dst;
-    if (hd < p.q_heads) {
-      src = p.q + b * p.q_bs + s * p.q_ts + (int64_t)hd * p.head;
-      dst = p.qo + b * p.qo_bs + s * p.qo_ts + (int64_t)hd * p.head;
-    } else {
-      hd -= p.q_heads;
-      src = p.k + b * p.k_bs + s * p.k_ts + (int64_t)hd * p.head;
-      dst = p.ko + b * p.ko_bs + s * p.ko_ts + (int64_t)hd * p.head;
+  for (int i0 = threadIdx.x; i0 < total; i0 += 256 * U) {
+    Item x[U];
+    const float2* cs[U];
+    bf16_t* dst[U];
+    int it[U];                                   // of the head: < n_turn rotated, else copied
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * 256, total - 1);
+      const int t = p.tok_per_block == 1 ? 0 : by(i, p.items_magic);
+      const int in_tok = i - t * p.items;
+      int hd = by(in_tok, p.head_magic);
+      it[u] = in_tok - hd * p.per_head;
+      const bool is_k = hd >= p.q_heads;
+      hd -= is_k ? p.q_heads : 0;
+      const int at = it[u] < p.n_turn ? it[u] * Item::W : p.rot + (it[u] - p.n_turn) * V;
+      const bf16_t* src = (is_k ? p.k + at_k[t] : p.q + at_q[t]) + (int64_t)hd * p.head + at;
+      dst[u] = (is_k ? p.ko + at_ko[t] : p.qo + at_qo[t]) + (int64_t)hd * p.head + at;
+      cs[u] = turn_cs + t * half + (NEOX ? at : at >> 1);
+      const bool turned = it[u] < p.n_turn;
+      Item::get(x[u].a, src, turned ? 2 : 1);
+      if (NEOX) Item::get(x[u].b, src + (turned ? half : 0), 1);
     }
-    const float2* cs = turn_cs + t * half;
-    if (it >= p.n_turn) {      // behind the rotated part: copied as it is
-      const int at = p.rot + (it - p.n_turn) * V;
-      if constexpr (V == 1) dst[at] = src[at];
-      else *reinterpret_cast<vec_t*>(dst + at) = *reinterpret_cast<const vec_t*>(src + at);
-    } else if constexpr (NEOX) {
-      const int at = it * V;
-      uint16_t lo[V], hi[V];
-      if constexpr (V == 1) {
-        lo[0] = src[at];
-        hi[0] = src[half + at];
-      } else {
-        *reinterpret_cast<vec_t*>(lo) = *reinterpret_cast<const vec_t*>(src + at);
-        *reinterpret_cast<vec_t*>(hi) = *reinterpret_cast<const vec_t*>(src + half + at);
-      }
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float a = bf2f(lo[j]), c = bf2f(hi[j]);
-        const float2 r = cs[at + j];
-        lo[j] = f2bf(a * r.x - c * r.y);
-        hi[j] = f2bf(c * r.x + a * r.y);
-      }
-      if constexpr (V == 1) {
-        dst[at] = lo[0];
-        dst[half + at] = hi[0];
-      } else {
-        *reinterpret_cast<vec_t*>(dst + at) = *reinterpret_cast<const vec_t*>(lo);
-        *reinterpret_cast<vec_t*>(dst + half + at) = *reinterpret_cast<const vec_t*>(hi);
-      }
-    } else {
-      constexpr int W = V == 1 ? 2 : V;      // V == 1: one pair, element by element (odd strides)
-      const int at = it * W;
-      uint16_t x[W];
-      if constexpr (V == 1) {
-        x[0] = src[at];
-        x[1] = src[at + 1];
-      } else {
-        *reinterpret_cast<vec_t*>(x) = *reinterpret_cast<const vec_t*>(src + at);
-      }
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * 256 >= total) break;
+      if (it[u] < p.n_turn) {
+        if constexpr (NEOX) {
 #pragma unroll
-      for (int j = 0; j < W / 2; ++j) {
-        const float a = bf2f(x[2 * j]), c = bf2f(x[2 * j + 1]);
-        const float2 r = cs[at / 2 + j];
-        x[2 * j] = f2bf(a * r.x - c * r.y);
-        x[2 * j + 1] = f2bf(c * r.x + a * r.y);
-      }
-      if constexpr (V == 1) {
-        dst[at] = x[0];
-        dst[at + 1] = x[1];
+          for (int j = 0; j < V; ++j) {
+            const float a = bf2f(x[u].a[j]), c = bf2f(x[u].b[j]);
+            const float2 r = cs[u][j];
+            x[u].a[j] = f2bf(a * r.x - c * r.y);
+            x[u].b[j] = f2bf(c * r.x + a * r.y);
+          }
+          Item::put(dst[u] + half, x[u].b, 1);
+        } else {
+#pragma unroll
+          for (int j = 0; j < Item::W / 2; ++j) {
+            const float a = bf2f(x[u].a[2 * j]), c = bf2f(x[u].a[2 * j + 1]);
+            const float2 r = cs[u][j];
+            x[u].a[2 * j] = f2bf(a * r.x - c * r.y);
+            x[u].a[2 * j + 1] = f2bf(c * r.x + a * r.y);
+          }
+        }
+        Item::put(dst[u], x[u].a, 2);
       } else {
-        *reinterpret_cast<vec_t*>(dst + at) = *reinterpret_cast<const vec_t*>(x);
+        Item::put(dst[u], x[u].a, 1);
       }
     }
   }
@@ -372,7 +392,8 @@ int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, c
   if (!turns || (reinterpret_cast<uintptr_t>(turns) & 7) || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out))) return FDM_ERR_INVALID;
   if (positions && position_bytes != 4 && position_bytes != 8) return FDM_ERR_INVALID;
   if (positions && (reinterpret_cast<uintptr_t>(positions) & (position_bytes - 1))) return FDM_ERR_INVALID;
-  if (rot_dim > 2 * ROPE_MAX_HALF || seq > 0x7fffffff || batch > 0x7fffffff || (int64_t)(q_heads + k_heads) * head_size > (1 << 24))
+  if (rot_dim > 2 * ROPE_MAX_HALF || seq > 0x7fffffff || batch > 0x7fffffff || head_size > 1024 ||
+      ((int64_t)q_heads + k_heads) * head_size > (1 << 22))
     return FDM_ERR_UNSUPPORTED;
   uintptr_t at = 0;
   int64_t strides = 0;
@@ -406,6 +427,9 @@ int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, c
   int tok = 1024 / a.items;
   tok = tok < 1 ? 1 : tok > ROPE_MAX_TOK ? ROPE_MAX_TOK : tok;
   a.tok_per_block = tok;
+  // i / d as the high word of i * ceil(2^32 / d), exact while i * d < 2^32: with several tokens i < 1024; within a token i < 2^22 and d <= 1024
+  a.items_magic = a.items == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + a.items - 1) / a.items);
+  a.head_magic = a.per_head == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + a.per_head - 1) / a.per_head);
   const int64_t grid = (a.tokens + tok - 1) / tok;
   if (grid > 0x7fffffff) return FDM_ERR_UNSUPPORTED;
   const size_t lds = (size_t)tok * half * sizeof(float2);

@@ -97,28 +97,36 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     x, residual: [rows, width] bf16, rows may be column slices of wider matrices.  Returns (bf16 y | None, Quantized | None, h | None) like ln_modulate.
     residual_out: where h goes (may be `residual` or `x` itself: in place).  residual=None: the norm of x alone, h is None.
     e4m3: scale = max|y| / 448; int8: asymmetric (scale, azp), as the row quantisers."""
-    N.need_gpu("add_rms_norm", x, residual, weight, residual_out)
+    gpu = N.gpu_of("add_rms_norm", x, residual, weight, residual_out)
     assert x.ndim == 2 and x.dtype == BF16 and weight.dtype == BF16, "add_rms_norm: x [rows, width] and weight in bf16"
-    rows, width = x.shape
+    rows, width = shape = x.shape
     assert 0 < width <= 65536, "add_rms_norm: 1 <= width <= 65536"
     assert quant in QUANT_MODE, "add_rms_norm: quant None, torch.float8_e4m3fn or torch.int8"
-    assert weight.is_contiguous() and weight.numel() == width, "add_rms_norm: weight [width]"
+    assert weight.numel() == width and weight.is_contiguous(), "add_rms_norm: weight [width]"
     xs = N.row_stride(x, "add_rms_norm")
-    rs = hs = 0
+    rs = hs = residual_ptr = h_ptr = 0
     if residual is not None:
-        assert residual.shape == x.shape and residual.dtype == BF16, "add_rms_norm: residual as x"
+        assert residual.shape == shape and residual.dtype == BF16, "add_rms_norm: residual as x"
+        rs = N.row_stride(residual, "add_rms_norm")
         if residual_out is None:
-            residual_out = torch.empty((rows, width), device=x.device, dtype=BF16)
-        assert residual_out.shape == x.shape and residual_out.dtype == BF16, "add_rms_norm: residual_out as x"
-        rs, hs = N.row_stride(residual, "add_rms_norm"), N.row_stride(residual_out, "add_rms_norm")
+            residual_out, hs = x.new_empty(shape), width
+        else:
+            assert residual_out.shape == shape and residual_out.dtype == BF16, "add_rms_norm: residual_out as x"
+            hs = N.row_stride(residual_out, "add_rms_norm")
+        residual_ptr, h_ptr = residual.data_ptr(), residual_out.data_ptr()
     else:
         assert residual_out is None, "add_rms_norm: residual_out without residual"
-    qz = _alloc_q(rows, width, quant, x.device) if quant is not None else None
-    out = torch.empty((rows, width), device=x.device, dtype=BF16) if quant is None else None
-    with N.on_device(x):
-        N.check(N.lib().fdm_add_rms_norm(N.ptr(out), N.ptr(qz.q) if qz else None, N.ptr(qz.scale) if qz else None,
-                                         N.ptr(qz.azp) if qz else None, QUANT_MODE[quant], N.ptr(x), N.ptr(residual), N.ptr(weight),
-                                         N.ptr(residual_out), rows, width, xs, rs, hs, eps, N.stream(x.device.index)), "add_rms_norm")
+    out = qz = None
+    out_ptr = q_ptr = scale_ptr = azp_ptr = 0
+    if quant is None:
+        out = x.new_empty(shape)
+        out_ptr = out.data_ptr()
+    else:
+        qz = Quantized(x.new_empty(shape, dtype=quant), x.new_empty((rows, 1), dtype=torch.float32),
+                       x.new_empty((rows, 1), dtype=torch.int32) if quant == torch.int8 else None)
+        q_ptr, scale_ptr, azp_ptr = qz.q.data_ptr(), qz.scale.data_ptr(), 0 if qz.azp is None else qz.azp.data_ptr()
+    N.launch("add_rms_norm", gpu, N.lib().fdm_add_rms_norm, out_ptr, q_ptr, scale_ptr, azp_ptr, QUANT_MODE[quant], x.data_ptr(), residual_ptr, weight.data_ptr(),
+             h_ptr, rows, width, xs, rs, hs, eps)
     return out, qz, residual_out
 
 

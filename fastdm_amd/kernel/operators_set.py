@@ -51,6 +51,23 @@ def rotary_pos_embedding(query: torch.Tensor, key: torch.Tensor, head_size: int,
     return
 
 
+def _rotary_side(x, out, B, S, head_size, what):
+    """(out, heads, batch and token strides of x and of out) of rotary_positions' query or key."""
+    assert x.ndim == 3 and x.dtype == BF16, f"rotary_positions: {what} [B, S, heads * head_size] in bf16"
+    b, s, width = shape = x.shape
+    assert b == B and s == S and width % head_size == 0, f"rotary_positions: {what}'s shape"
+    x_bs, x_ts, x_es = x.stride()
+    assert x_es == 1, f"rotary_positions: {what}'s tokens must be dense"
+    if out is None:
+        return x.new_empty(shape), width // head_size, x_bs, x_ts, S * width, width
+    assert out.shape == shape and out.dtype == BF16, f"rotary_positions: {what}_out as {what}"
+    o_bs, o_ts, o_es = out.stride()
+    assert o_es == 1, f"rotary_positions: {what}_out's tokens must be dense"
+    assert (S <= 1 or o_ts >= width) and (B <= 1 or o_bs >= width), f"rotary_positions: {what}_out overlaps itself"
+    assert out.data_ptr() != x.data_ptr() or (x_bs, x_ts) == (o_bs, o_ts), f"rotary_positions: {what} in place needs the same strides"
+    return out, width // head_size, x_bs, x_ts, o_bs, o_ts
+
+
 def rotary_positions(query: torch.Tensor, key: Optional[torch.Tensor], head_size: int, frequencies, positions: Optional[torch.Tensor] = None,
                      is_neox: bool = False, query_out: Optional[torch.Tensor] = None,
                      key_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
@@ -60,43 +77,29 @@ def rotary_positions(query: torch.Tensor, key: Optional[torch.Tensor], head_size
     place and the result is rounded once.  is_neox: pairs (i, i + rotary_dim / 2) instead of (2i, 2i + 1).  Inputs may be slices of a fused
     projection (any batch and token strides); returns (query_out, key_out), new tensors unless given -- `query` / `key` themselves for in place,
     a cache's slice for a key that is stored there."""
-    N.need_gpu("rotary_positions", query, key, positions, query_out, key_out, frequencies.turns)
+    gpu = N.gpu_of("rotary_positions", query, key, positions, query_out, key_out, frequencies.turns)
     rot = frequencies.rotary_dim
     assert rot <= head_size, "rotary_positions: rotary_dim is larger than the head"
     assert query.ndim == 3, "rotary_positions: query [B, S, heads * head_size]"
     B, S, _ = query.shape
-
-    def side(x, out, what):
-        assert x.ndim == 3 and x.dtype == BF16, f"rotary_positions: {what} [B, S, heads * head_size] in bf16"
-        width = x.shape[2]
-        assert x.shape[0] == B and x.shape[1] == S and width % head_size == 0, f"rotary_positions: {what}'s shape"
-        if out is None:
-            out = torch.empty((B, S, width), device=x.device, dtype=BF16)
-        assert out.shape == x.shape and out.dtype == BF16, f"rotary_positions: {what}_out as {what}"
-        (x_bs, x_ts, x_es), (o_bs, o_ts, o_es) = x.stride(), out.stride()
-        assert x_es == 1 and o_es == 1, f"rotary_positions: {what}'s tokens must be dense"
-        assert (S <= 1 or o_ts >= width) and (B <= 1 or o_bs >= width), f"rotary_positions: {what}_out overlaps itself"
-        assert x_bs >= 0 and x_ts >= 0, f"rotary_positions: {what}'s strides"
-        assert out.data_ptr() != x.data_ptr() or (x_bs, x_ts) == (o_bs, o_ts), f"rotary_positions: {what} in place needs the same strides"
-        return out, width // head_size, x_bs, x_ts, o_bs, o_ts
-
-    query_out, q_heads, q_bs, q_ts, qo_bs, qo_ts = side(query, query_out, "query")
-    k_heads = k_bs = k_ts = ko_bs = ko_ts = 0
+    query_out, q_heads, *q_strides = _rotary_side(query, query_out, B, S, head_size, "query")
+    k_heads = key_ptr = key_out_ptr = 0
+    k_strides = (0, 0, 0, 0)
     if key is not None:
-        key_out, k_heads, k_bs, k_ts, ko_bs, ko_ts = side(key, key_out, "key")
+        key_out, k_heads, *k_strides = _rotary_side(key, key_out, B, S, head_size, "key")
+        key_ptr, key_out_ptr = key.data_ptr(), key_out.data_ptr()
     else:
         assert key_out is None, "rotary_positions: key_out without key"
-    p_bs = p_ts = p_bytes = 0
+    p_ptr = p_bs = p_ts = p_bytes = 0
     if positions is not None:
         assert positions.dtype in (torch.int32, torch.int64), "rotary_positions: positions int32 or int64"
         assert positions.shape == (S,) or positions.shape == (B, S), "rotary_positions: positions [S] or [B, S]"
-        p_bytes, p_ts = positions.element_size(), positions.stride(-1)
-        p_bs = positions.stride(0) if positions.ndim == 2 else 0
-    with N.on_device(query):
-        N.check(N.lib().fdm_rope_positions(N.ptr(query_out), N.ptr(key_out), N.ptr(query), N.ptr(key), frequencies.turns.data_ptr(),
-                                           N.ptr(positions), p_bytes, p_bs, p_ts, B, S, q_heads, k_heads, head_size, rot, q_bs, q_ts, k_bs, k_ts,
-                                           qo_bs, qo_ts, ko_bs, ko_ts, frequencies.amplitude, int(bool(is_neox)), N.stream(query.device.index)),
-                "rotary_positions")
+        p_ptr, p_bytes = positions.data_ptr(), positions.element_size()
+        *p_bs, p_ts = positions.stride()
+        p_bs = p_bs[0] if p_bs else 0
+    N.launch("rotary_positions", gpu, N.lib().fdm_rope_positions, query_out.data_ptr(), key_out_ptr, query.data_ptr(), key_ptr, frequencies.turns.data_ptr(),
+             p_ptr, p_bytes, p_bs, p_ts, B, S, q_heads, k_heads, head_size, rot, q_strides[0], q_strides[1], k_strides[0], k_strides[1],
+             q_strides[2], q_strides[3], k_strides[2], k_strides[3], frequencies.amplitude, 1 if is_neox else 0)
     return query_out, key_out
 
 
@@ -262,33 +265,38 @@ def window_scaled_dot_product_attention(query: torch.Tensor, key: torch.Tensor, 
     row t is at place kv_len - q_len + t and sees key j iff j <= place and (place - j < window or j < sinks).  q_lens / kv_lens: int32 [B] on the GPU
     for padded batches and part-filled caches (default Sq / Sk; lengths outside 0 .. Sq / Sk count as the nearest).  Rows past q_len and rows that see
     nothing are zeros; keys past kv_len and keys no row sees may hold anything.  Prompts, chunks behind a cache, and single tokens (Sq = 1)."""
-    N.need_gpu("window_scaled_dot_product_attention", query, key, value, q_lens, kv_lens)
+    name = "window_scaled_dot_product_attention"
+    gpu = N.gpu_of(name, query, key, value, q_lens, kv_lens)
     assert query.dtype == BF16 and key.dtype == BF16 and value.dtype == BF16, "window_scaled_dot_product_attention: bf16 only"
     assert query.ndim == 3 and key.ndim == 3 and key.shape == value.shape, "window_scaled_dot_product_attention: [B, S, heads * head_dim]"
-    B, Sq, width = query.shape
-    Sk = key.shape[1]
+    B, Sq, width = shape = query.shape
+    Bk, Sk, kv_width = key.shape
     assert head_dim in (64, 128), "window_scaled_dot_product_attention: head_dim 64 or 128"
     assert num_kv_heads > 0 and num_q_heads % num_kv_heads == 0, "window_scaled_dot_product_attention: q heads are a multiple of the kv heads"
-    assert width == num_q_heads * head_dim and key.shape[2] == num_kv_heads * head_dim and key.shape[0] == B, "window_scaled_dot_product_attention: shapes"
+    assert width == num_q_heads * head_dim and kv_width == num_kv_heads * head_dim and Bk == B, "window_scaled_dot_product_attention: shapes"
     assert window >= 1 and sinks >= 0, "window_scaled_dot_product_attention: window >= 1, sinks >= 0"
-    for t in (query, key, value):
-        assert t.stride(2) == 1, "window_scaled_dot_product_attention: tokens must be dense"
-    for lens in (q_lens, kv_lens):
-        assert lens is None or (lens.dtype == torch.int32 and lens.shape == (B,) and lens.is_contiguous()), "window_scaled_dot_product_attention: lengths int32 [B]"
+    (q_bs, q_ts, q_es), (k_bs, k_ts, k_es), (v_bs, v_ts, v_es) = query.stride(), key.stride(), value.stride()
+    assert q_es == 1 and k_es == 1 and v_es == 1, "window_scaled_dot_product_attention: tokens must be dense"
+    q_lens_ptr = kv_lens_ptr = 0
+    if q_lens is not None:
+        assert q_lens.dtype == torch.int32 and q_lens.shape == (B,) and q_lens.is_contiguous(), "window_scaled_dot_product_attention: q_lens int32 [B]"
+        q_lens_ptr = q_lens.data_ptr()
+    if kv_lens is not None:
+        assert kv_lens.dtype == torch.int32 and kv_lens.shape == (B,) and kv_lens.is_contiguous(), "window_scaled_dot_product_attention: kv_lens int32 [B]"
+        kv_lens_ptr = kv_lens.data_ptr()
     if scale is None:
         scale = head_dim ** -0.5
     assert 0.0 < scale < 3e38, "window_scaled_dot_product_attention: scale > 0"
-    out = torch.empty((B, Sq, width), device=query.device, dtype=BF16)
-    need = _window_workspace(B, Sq, Sk, num_q_heads, num_kv_heads, head_dim, window, sinks)
-    ws = torch.empty(need, device=query.device, dtype=torch.uint8) if need else None      # of this call alone: a captured graph's comes from its own pool
-    (q_bs, q_ts, _), (k_bs, k_ts, _), (v_bs, v_ts, _) = query.stride(), key.stride(), value.stride()
-    with N.on_device(query):
-        N.check(N.lib().fdm_attn_window(N.ptr(out), N.ptr(query), N.ptr(key), N.ptr(value), N.ptr(q_lens), N.ptr(kv_lens), B, Sq, Sk, num_q_heads,
-                                        num_kv_heads, head_dim, q_bs, q_ts, k_bs, k_ts, v_bs, v_ts, Sq * width, width, scale, window, sinks, N.ptr(ws), need,
-                                        N.stream(query.device.index)), "window_scaled_dot_product_attention")
+    out = query.new_empty(shape)
+    need = _window_workspace(gpu, B, Sq, Sk, num_q_heads, num_kv_heads, head_dim, window, sinks)
+    ws = query.new_empty(need, dtype=torch.uint8) if need else None      # of this call alone: a captured graph's comes from its own pool
+    N.launch(name, gpu, N.lib().fdm_attn_window, out.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(), q_lens_ptr, kv_lens_ptr, B, Sq, Sk,
+             num_q_heads, num_kv_heads, head_dim, q_bs, q_ts, k_bs, k_ts, v_bs, v_ts, Sq * width, width, scale, window, sinks,
+             0 if ws is None else ws.data_ptr(), need)
     return out
 
 
 @functools.lru_cache(maxsize=4096)
-def _window_workspace(*shape) -> int:
-    return int(N.lib().fdm_attn_window_workspace_bytes(*shape))
+def _window_workspace(gpu, *shape) -> int:
+    with torch.cuda.device(gpu):      # (it goes by the device's compute units)
+        return int(N.lib().fdm_attn_window_workspace_bytes(*shape))

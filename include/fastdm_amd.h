@@ -458,7 +458,7 @@ int fdm_add_rms_norm(void* out_bf16, void* out_q, float* out_scale, int32_t* out
  * rot_dim elements -- (2i, 2i + 1), or (i, i + rot_dim / 2) where is_neox -- turns by 2 pi * place * turns[i] and is scaled by amplitude; the rest of
  * the head is copied.  turns: fp64 [rot_dim / 2], turns per position; the angle's fraction of a turn is taken in 64 bits, sine and cosine in fp32.
  * positions: int32 / int64 (position_bytes 4 / 8) at positions[b * pos_batch_stride + s * pos_tok_stride], or NULL for 0 .. seq - 1.
- * rot_dim even, <= 256.  k_heads == 0: q alone.                                                                                        */
+ * rot_dim even, <= 256; head_size <= 1024, at most 2^22 elements per token.  k_heads == 0: q alone.                                        */
 int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, const void* turns, const void* positions, int position_bytes,
                        int64_t pos_batch_stride, int64_t pos_tok_stride, int64_t batch, int64_t seq, int q_heads, int k_heads, int head_size,
                        int rot_dim, int64_t q_batch_stride, int64_t q_tok_stride, int64_t k_batch_stride, int64_t k_tok_stride,

@@ -133,3 +133,8 @@ def test_window_attention_refuses_cpu_tensors():
     x = torch.zeros(1, 4, 64, dtype=BF16)
     with pytest.raises(RuntimeError, match="GPU"):
         window_scaled_dot_product_attention(x, x, x, 1, 1, 64, 2)
+
+
+@pytest.mark.parametrize("kw,code", [(dict(head=1032, rot=64), -2), (dict(hq=65536, hk=1, head=64), -2)])
+def test_rope_positions_c_entry_refuses_what_its_numbers_do_not_hold(kw, code):
+    assert c_rope(**kw) == code

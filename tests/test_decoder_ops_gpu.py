@@ -154,7 +154,7 @@ def rope64(x, head, freqs, positions, is_neox):
 
 
 @pytest.mark.parametrize("is_neox", [False, True])
-@pytest.mark.parametrize("head,rot", [(128, 128), (64, 32), (64, 64), (80, 20), (96, 24), (256, 256), (256, 64), (10, 6), (7, 2), (128, 12)])
+@pytest.mark.parametrize("head,rot", [(128, 128), (64, 32), (64, 64), (80, 20), (96, 24), (256, 256), (256, 64), (10, 6), (7, 2), (128, 12), (8, 8), (2, 2), (1024, 16), (520, 250)])
 @pytest.mark.parametrize("B,S,Hq,Hk", [(1, 1, 4, 1), (3, 37, 8, 2), (2, 5, 1, 1)])
 def test_rotary_positions(B, S, Hq, Hk, head, rot, is_neox):
     from fastdm_amd.kernel.operators_set import rotary_positions
@@ -458,3 +458,35 @@ def test_window_attention_behind_offsets_over_32_bits():
     got = attend(q, k, v, Hq, Hk, D, 500)
     want, tol = window64(q, k[:, -600:], v[:, -600:], Hq, Hk, D, 500, 0)
     assert_within(got, want, tol, "far keys")
+
+
+@pytest.mark.parametrize("bad", [None, float("nan")])
+@pytest.mark.parametrize("B,S,L,Hq,Hk,D,window,sinks", [(8, 300, 300, 12, 12, 64, 100, 5), (8, 300, 420, 12, 12, 128, 100, 70), (3, 411, 411, 56, 8, 128, 64, 1),
+                                                        (5, 260, 2600, 4, 2, 128, 2100, 130), (1, 515, 3000, 16, 4, 128, 2500, 0), (9, 130, 130, 48, 16, 64, 200, 0)])
+def test_window_attention_of_many_blocks_and_of_long_lists(B, S, L, Hq, Hk, D, window, sinks, bad):
+    """Row blocks that fill the chip, and long lists of few blocks: ragged, with neighbours that are not numbers."""
+    g = gen(B * S + L + D)
+    q, k, v = randn(g, B, S, Hq * D, scale=1.5), randn(g, B, L, Hk * D), randn(g, B, L, Hk * D)
+    qn = lens(*[S - 17 * b for b in range(B)])
+    kv = lens(*[L - 29 * b for b in range(B)])
+    clean = check_window(q, k, v, Hq, Hk, D, window, sinks, q_lens=qn, kv_lens=kv)
+    if bad is None:
+        check_window(q, k, v, Hq, Hk, D, window, sinks)
+        return
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    j = L - S // 2
+    sees = []
+    for b in range(B):
+        kv_len, q_len = L - 29 * b, S - 17 * b
+        k[b, kv_len:], v[b, kv_len:] = bad, bad
+        front = max(sinks, kv_len - q_len - window + 1)
+        k[b, sinks:front], v[b, sinks:front] = bad, bad
+        row = torch.arange(S, device="cuda")
+        place = kv_len - q_len + row
+        sees.append((row < q_len) & (place >= j) & ((place < j + window) | (j < sinks)) if j < kv_len else torch.zeros(S, dtype=torch.bool, device="cuda"))
+        if j < kv_len:
+            v[b, j, 5::D] = bad                       # one element of every kv head's value
+    got = attend(q, k, v, Hq, Hk, D, window, sinks=sinks, q_lens=qn, kv_lens=kv)
+    hit = torch.stack(sees)[:, :, None] & (torch.arange(Hq * D, device="cuda") % D == 5)
+    assert hit.any() and torch.isnan(got[hit]).all()
+    assert torch.equal(got[~hit], clean[~hit])
