@@ -261,7 +261,7 @@ def window_scaled_dot_product_attention(query: torch.Tensor, key: torch.Tensor, 
                                         window: int, sinks: int = 0, scale: Optional[float] = None, q_lens: Optional[torch.Tensor] = None,
                                         kv_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention whose queries see the last `window` keys (their own among them) and the first `sinks`: query [B, Sq, Hq*D], key / value
-    [B, Sk, Hkv*D] (a cache, or slices of one: any batch and token strides), [B, Sq, Hq*D] out.  The queries of a sequence are the last of its tokens:
+    [B, Sk, Hkv*D] (a cache, or slices of one: batch and token strides of any multiples of 8, 16-byte aligned), [B, Sq, Hq*D] out.  The queries of a sequence are the last of its tokens:
     row t is at place kv_len - q_len + t and sees key j iff j <= place and (place - j < window or j < sinks).  q_lens / kv_lens: int32 [B] on the GPU
     for padded batches and part-filled caches (default Sq / Sk; lengths outside 0 .. Sq / Sk count as the nearest).  Rows past q_len and rows that see
     nothing are zeros; keys past kv_len and keys no row sees may hold anything.  Prompts, chunks behind a cache, and single tokens (Sq = 1)."""
@@ -275,8 +275,15 @@ def window_scaled_dot_product_attention(query: torch.Tensor, key: torch.Tensor, 
     assert num_kv_heads > 0 and num_q_heads % num_kv_heads == 0, "window_scaled_dot_product_attention: q heads are a multiple of the kv heads"
     assert width == num_q_heads * head_dim and kv_width == num_kv_heads * head_dim and Bk == B, "window_scaled_dot_product_attention: shapes"
     assert window >= 1 and sinks >= 0, "window_scaled_dot_product_attention: window >= 1, sinks >= 0"
+    window, sinks = max(1, min(window, Sk)), min(sinks, Sk)              # (the same keys; any whole number fits the entry's 64 bits)
     (q_bs, q_ts, q_es), (k_bs, k_ts, k_es), (v_bs, v_ts, v_es) = query.stride(), key.stride(), value.stride()
     assert q_es == 1 and k_es == 1 and v_es == 1, "window_scaled_dot_product_attention: tokens must be dense"
+    if B <= 1:                                                           # (the stride of an axis of one is any number)
+        q_bs = k_bs = v_bs = 0
+    if Sq <= 1:
+        q_ts = 0
+    if Sk <= 1:
+        k_ts = v_ts = 0
     q_lens_ptr = kv_lens_ptr = 0
     if q_lens is not None:
         assert q_lens.dtype == torch.int32 and q_lens.shape == (B,) and q_lens.is_contiguous(), "window_scaled_dot_product_attention: q_lens int32 [B]"

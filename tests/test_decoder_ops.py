@@ -138,3 +138,32 @@ def test_window_attention_refuses_cpu_tensors():
 @pytest.mark.parametrize("kw,code", [(dict(head=1032, rot=64), -2), (dict(hq=65536, hk=1, head=64), -2)])
 def test_rope_positions_c_entry_refuses_what_its_numbers_do_not_hold(kw, code):
     assert c_rope(**kw) == code
+
+
+def test_launch_goes_to_the_tensors_device(monkeypatch):
+    """A kernel is launched with its tensors' GPU as the current device and on that GPU's stream, whichever was current."""
+    seen, current = [], [0]
+
+    class device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+
+    monkeypatch.setattr(N, "_current_device", lambda: current[0])
+    monkeypatch.setattr(N, "stream", lambda index: 100 + index)
+    monkeypatch.setattr(torch.cuda, "device", device)
+
+    def entry(*args):
+        seen.append((current[0], args))
+        return 0
+
+    N.launch("x", 0, entry, 1)
+    N.launch("x", 3, entry, 2)
+    assert seen == [(0, (1, 100)), (3, (2, 103))] and current[0] == 0
+    with pytest.raises(RuntimeError, match="x failed: unsupported"):
+        N.launch("x", 0, lambda *a: -2)

@@ -241,7 +241,7 @@ def window64(q, k, v, Hq, Hk, D, window, sinks, scale=None, q_lens=None, kv_lens
     """In 64 bits, one sequence and kv head at a time, over the visible keys alone; and the tolerance element by element."""
     B, S, _ = q.shape
     L = k.shape[1]
-    scale = D ** -0.5 if scale is None else scale
+    scale, window, sinks = D ** -0.5 if scale is None else scale, min(window, L + 1), min(sinks, L)
     out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
     tol = torch.zeros_like(out)
     G = Hq // Hk
@@ -490,3 +490,171 @@ def test_window_attention_of_many_blocks_and_of_long_lists(B, S, L, Hq, Hk, D, w
     hit = torch.stack(sees)[:, :, None] & (torch.arange(Hq * D, device="cuda") % D == 5)
     assert hit.any() and torch.isnan(got[hit]).all()
     assert torch.equal(got[~hit], clean[~hit])
+
+
+def test_window_attention_takes_any_stride_of_an_axis_of_one():
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    g = gen(21)
+    q, k, v = randn(g, 1, 1, 256), randn(g, 1, 50, 128), randn(g, 1, 50, 128)
+    want = check_window(q, k, v, 4, 2, 64, 1 << 70, 1 << 70)
+    odd = [torch.as_strided(t, t.shape, (t.stride(0) + 3, t.stride(1) if t.shape[1] > 1 else 5, 1)) for t in (q, k, v)]
+    assert torch.equal(attend(*odd, 4, 2, 64, 50, sinks=3), want)
+    one = attend(q, torch.as_strided(k, (1, 1, 128), (7, 9, 1)), torch.as_strided(v, (1, 1, 128), (7, 9, 1)), 4, 2, 64, 1)
+    assert torch.equal(one.view(2, 2, 64), v[0, 0].view(2, 1, 64).expand(2, 2, 64))
+
+
+# ================================================================================================ together
+class DecoderAttention:
+    """The attention half of a decoder layer as a program that serves runs it: the residual's addition and norm into e4m3, the fused W8A8 projection, rotary
+    positions of q and of k straight into the cache, attention over the cache."""
+
+    def __init__(self, seed, width, Hq, Hk, D, window, sinks, batch, room):
+        from fastdm_amd.kernel.operators_set import quantize_to_fp8
+        from fastdm_amd.layer.embeddings import RotaryFrequencies
+        g = gen(seed)
+        self.Hq, self.Hk, self.D, self.window, self.sinks = Hq, Hk, D, window, sinks
+        self.weight = (1 + 0.1 * torch.randn(width, generator=g, device="cuda")).to(BF16)
+        self.proj, self.proj_scale = quantize_to_fp8(randn(g, (Hq + 2 * Hk) * D, width, scale=width ** -0.5))
+        self.freqs = RotaryFrequencies(D, base=500000.0, scaling="yarn", factor=4.0, original_length=64, device="cuda")
+        self.k, self.v = (torch.full((batch, room, Hk * D), float("nan"), device="cuda", dtype=BF16) for _ in range(2))
+
+    def __call__(self, x, residual, at, q_lens=None, kv_lens=None):
+        """Tokens at .. at + S - 1 of every sequence; returns (attention's output, the new residual, q)."""
+        from fastdm_amd.kernel.fused import add_rms_norm
+        from fastdm_amd.kernel.operators_set import fp8_matmul, rotary_positions, window_scaled_dot_product_attention
+        B, S, width = x.shape
+        qw, kw = self.Hq * self.D, self.Hk * self.D
+        _, z, h = add_rms_norm(x.view(B * S, width), residual.view(B * S, width), self.weight, 1e-6, quant=FP8)
+        qkv = fp8_matmul(z.q, self.proj.t(), z.scale, self.proj_scale, BF16).view(B, S, qw + 2 * kw)
+        positions = torch.arange(at, at + S, device="cuda")
+        q, _ = rotary_positions(qkv[..., :qw], qkv[..., qw:qw + kw], self.D, self.freqs, positions, is_neox=True, key_out=self.k[:, at:at + S])
+        self.v[:, at:at + S] = qkv[..., qw + kw:]
+        o = window_scaled_dot_product_attention(q, self.k[:, :at + S], self.v[:, :at + S], self.Hq, self.Hk, self.D, self.window, sinks=self.sinks,
+                                                q_lens=q_lens, kv_lens=kv_lens)
+        return o, h.view(B, S, width), q
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_decoder_attention_prompt_then_single_tokens(D):
+    """A prompt in one call, in chunks, and token by token give the same rows: the row operators bit for bit, attention within its tolerance; the
+    cache is NaN where nothing was written yet."""
+    B, S, width, Hq, Hk, window, sinks = 2, 150, 512, 8, 2, 48, 3
+    g = gen(31)
+    x, residual = randn(g, B, S, width), randn(g, B, S, width, scale=3.0)
+    whole = DecoderAttention(5, width, Hq, Hk, D, window, sinks, B, S)
+    o, h, q = whole(x, residual, 0)
+    want, tol = window64(q, whole.k, whole.v, Hq, Hk, D, window, sinks)
+    assert_within(o, want, tol, "prompt")
+    for sizes in ([100, 33, 17], [140] + [1] * 10):
+        parts, at = DecoderAttention(5, width, Hq, Hk, D, window, sinks, B, S), 0
+        for n in sizes:
+            got, hn, qn = parts(x[:, at:at + n].contiguous(), residual[:, at:at + n].contiguous(), at)
+            assert torch.equal(hn, h[:, at:at + n])
+            # the projection's kernel goes by its number of rows: its sums may be taken in another order, so its rows are compared through attention alone
+            w, t = window64(qn, parts.k[:, :at + n], parts.v[:, :at + n], Hq, Hk, D, window, sinks)
+            assert_within(got, w, t, f"{n} tokens at {at}")
+            at += n
+        assert torch.isfinite(parts.k).all() and torch.isfinite(parts.v).all()
+
+
+def test_decoder_attention_step_in_a_graph():
+    """One token's step captured once and replayed for growing sequences (lengths and positions are device tensors), eager work and waits between."""
+    from fastdm_amd.kernel.fused import add_rms_norm
+    from fastdm_amd.kernel.operators_set import rotary_positions, window_scaled_dot_product_attention
+    from fastdm_amd.layer.embeddings import RotaryFrequencies
+    B, Hq, Hk, D, room, width = 3, 8, 2, 64, 900, 512
+    g = gen(41)
+    k, v = randn(g, B, room, Hk * D), randn(g, B, room, Hk * D)
+    x, residual = randn(g, B, width), randn(g, B, width)
+    weight = randn(g, width)
+    freqs = RotaryFrequencies(D, device="cuda")
+    kv = lens(600, 1, 300)
+    positions = torch.zeros(B, 1, dtype=torch.int64, device="cuda")
+
+    def step():
+        y, _, h = add_rms_norm(x, residual, weight, 1e-6)
+        q, _ = rotary_positions(y.view(B, 1, width), None, D, freqs, positions)
+        return h, q, window_scaled_dot_product_attention(q, k, v, Hq, Hk, D, 512, sinks=2, kv_lens=kv)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        x.copy_(randn(g, B, width))
+        kv.copy_(lens(600 + 7 * i, 1 + 250 * i, room - i))
+        positions.copy_(kv.long()[:, None] - 1)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(out, step()):
+            assert torch.equal(got, want)
+        want, tol = window64(out[1], k, v, Hq, Hk, D, 512, 2, kv_lens=kv)
+        assert_within(out[2], want, tol, "replayed")
+
+
+def test_calls_that_would_lose_a_gradient_and_mixed_devices_are_refused():
+    from fastdm_amd.kernel.fused import add_rms_norm
+    from fastdm_amd.kernel.operators_set import rotary_positions, window_scaled_dot_product_attention
+    from fastdm_amd.layer.embeddings import RotaryFrequencies
+    x = randn(gen(51), 4, 64)
+    w = torch.ones(64, device="cuda", dtype=BF16)
+    leaf = x.clone().requires_grad_()
+    freqs = RotaryFrequencies(64, device="cuda")
+    with pytest.raises(RuntimeError, match="forward only"):
+        add_rms_norm(leaf, None, w, 1e-6)
+    with pytest.raises(RuntimeError, match="forward only"):
+        rotary_positions(leaf[None], None, 64, freqs)
+    with pytest.raises(RuntimeError, match="forward only"):
+        window_scaled_dot_product_attention(x[None], leaf[None], x[None], 1, 1, 64, 4)
+    with torch.no_grad():
+        add_rms_norm(leaf, None, w, 1e-6)
+    with pytest.raises(RuntimeError, match="GPU"):
+        add_rms_norm(x, x.cpu(), w, 1e-6)
+    with pytest.raises(RuntimeError, match="GPU"):
+        rotary_positions(x[None], None, 64, RotaryFrequencies(64))
+    with pytest.raises(RuntimeError, match="GPU"):
+        window_scaled_dot_product_attention(x[None], x[None], x[None], 1, 1, 64, 4, kv_lens=torch.tensor([4], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("what", ["dtype", "shape", "heads", "head_dim", "window", "sinks", "scale", "lens dtype", "lens shape", "inner stride", "alignment", "batch"])
+def test_window_attention_refusals(what):
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    q, k = randn(gen(1), 2, 5, 256), randn(gen(2), 2, 9, 128)
+    a = dict(q=q, k=k, v=k, hq=4, hk=2, D=64, window=4, kw={})
+    change = {"dtype": dict(q=q.half()), "shape": dict(v=k[:, :8]), "heads": dict(hq=3, q=q[..., :192]), "head_dim": dict(D=32, hq=8, hk=4), "window": dict(window=0),
+              "sinks": dict(kw=dict(sinks=-1)), "scale": dict(kw=dict(scale=0.0)), "lens dtype": dict(kw=dict(kv_lens=torch.ones(2, dtype=torch.int64, device="cuda"))),
+              "lens shape": dict(kw=dict(q_lens=lens(1, 2, 3))), "inner stride": dict(q=q.transpose(1, 2).contiguous().transpose(1, 2)),
+              "alignment": dict(q=torch.cat((q, q), -1)[..., 4:260]), "batch": dict(k=k[:1], v=k[:1])}[what]
+    a.update(change)
+    with pytest.raises((AssertionError, RuntimeError)):
+        attend(a["q"], a["k"], a["v"], a["hq"], a["hk"], a["D"], a["window"], **a["kw"])
+
+
+@pytest.mark.parametrize("what", ["dtype", "width", "residual", "quant", "out without residual", "rows", "inner stride"])
+def test_add_rms_norm_refusals(what):
+    from fastdm_amd.kernel.fused import add_rms_norm
+    x, w = randn(gen(1), 6, 64), torch.ones(64, device="cuda", dtype=BF16)
+    call = {"dtype": lambda: add_rms_norm(x.float(), None, w, 1e-6), "width": lambda: add_rms_norm(x, None, w[:32], 1e-6), "residual": lambda: add_rms_norm(x, x[:3], w, 1e-6),
+            "quant": lambda: add_rms_norm(x, None, w, 1e-6, quant=torch.uint8), "out without residual": lambda: add_rms_norm(x, None, w, 1e-6, residual_out=x),
+            "rows": lambda: add_rms_norm(x[:1].expand(6, 64), None, w, 1e-6), "inner stride": lambda: add_rms_norm(randn(gen(1), 64, 6).t(), None, w, 1e-6)}[what]
+    with pytest.raises((AssertionError, RuntimeError)):
+        call()
+
+
+@pytest.mark.parametrize("what", ["rot", "shape", "head", "positions dtype", "positions shape", "out shape", "out overlaps", "in place strides", "key out without key"])
+def test_rotary_positions_refusals(what):
+    from fastdm_amd.kernel.operators_set import rotary_positions
+    from fastdm_amd.layer.embeddings import RotaryFrequencies
+    f = RotaryFrequencies(64, device="cuda")
+    q = randn(gen(1), 2, 6, 128)
+    call = {"rot": lambda: rotary_positions(q, None, 32, f), "shape": lambda: rotary_positions(q, q[:, :5], 64, f), "head": lambda: rotary_positions(q, None, 96, f),
+            "positions dtype": lambda: rotary_positions(q, None, 64, f, torch.zeros(6, device="cuda")), "positions shape": lambda: rotary_positions(q, None, 64, f, torch.zeros(5, dtype=torch.int64, device="cuda")),
+            "out shape": lambda: rotary_positions(q, None, 64, f, query_out=q[:, :5]), "out overlaps": lambda: rotary_positions(q, None, 64, f, query_out=q[:1].expand(2, 6, 128)),
+            "in place strides": lambda: rotary_positions(q, None, 64, f, query_out=torch.as_strided(q, (2, 6, 128), (128, 256, 1))),
+            "key out without key": lambda: rotary_positions(q, None, 64, f, key_out=q)}[what]
+    with pytest.raises((AssertionError, RuntimeError)):
+        call()
