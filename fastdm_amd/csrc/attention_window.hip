@@ -9,14 +9,21 @@
 //             multiplied.  A wave skips tiles none of its rows sees and masks element by element only where some row does not see some key.
 //   QK^T      swapped: S^T[key][q] = K . Q^T on v_mfma_f32_32x32x16_bf16: lane (q = lane & 31, h = lane >> 5) holds 16 of each 32 keys of ITS row.
 //   PV        O^T[d][q] += V^T[d][key] . P^T[key][q]: the S^T accumulator, converted pairwise to bf16, is the B operand as it is; V^T comes from the
-//             row-major tile through ds_read_b64_tr_b16.  P is rounded to bf16 (2^-9 of each weight, averaged over the keys; the row sums are those of
-//             the unrounded weights in fp32): the matrix core's operand type.
+//             row-major tile through ds_read_b64_tr_b16.  P is rounded to bf16 (at most 2^-8 of each weight, averaged over the keys; the row sums
+//             are those of the unrounded weights in fp32): the matrix core's operand type.
 //   softmax   one pass, running maximum and sum in fp32, exp2 domain, O and l rescaled only where a row's maximum grew by more than 2^8.
 //   waves     WR waves over rows (32 each) times WK waves over the keys of a tile, merged through LDS at the end (window_plan says which).  Where the blocks
 //             would not fill the chip, a block's tile list is cut into parts that run side by side and are merged by a second small launch.
 //   NaN       what a row does not see does not reach it, though 0 * NaN is NaN in the matrix core: masked scores are replaced, keys past kv_len are never
 //             read, values that no row of the block sees are zeroed in LDS, and a block that finds one that is not finite among those that only some
 //             rows see starts over: product with the finite values, and a second product of marks for the rows that see one that is not.
+//   bound     prompts: the matrix core and the softmax's VALU work behind it, which overlap across the two blocks of a CU only in part: 16384 tokens, 32/8
+//             heads x 128, window 4096: 945 - 990 us (by box) = 0.97 - 1.02 PFLOP/s of visible pairs, where a large bf16 product reaches 1.19; MFMA busy
+//             half of the cycles, LDS conflicts 0.  head_dim 64: VALU issue (32 exp2 of 4 issue slots each beside 16 MFMAs per tile).  Small grids: the
+//             chain of one block's tiles.  Single tokens: HBM, 16 sequences, window 4096: 54 us = 5.0 TB/s with the merge.
+//   tried     fragments read a group ahead behind scheduling fences (+3 .. 15 %, spills), a three- or four-deep ring (+1 / +12 % at head_dim 64), the
+//             next tile's scores under this tile's softmax (spills at head_dim 128; +10 % at 64), s_setprio around either phase (+1 %), the row sums by
+//             v_dot2 (0), 128-key tiles with eight waves (+6 %), 32-key tiles (+7 %): none of them stayed.
 #include <type_traits>
 #include "common.h"
 #include "attn_common.h"
@@ -41,8 +48,8 @@ struct WindowParams {
   float* ws_ml;         // ... [..][..][rows][2]: maximum (exp2 domain), sum
 };
 
-// ST: tiles in the LDS ring (one being worked on, the others on their way)
-template <int D, int WR, int WK, int KW, int ST, int OCC>
+// KW: keys per wave and tile; OCC: waves per SIMD that the registers have to do for.  LDS: two K / V tiles, one being worked on, one on its way
+template <int D, int WR, int WK, int KW, int OCC>
 __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const WindowParams p) {
   constexpr int NT = 64 * WR * WK, RB = 32 * WR, KT = KW * WK;
   constexpr int NKT = KW / 32;            // 32-key S^T tiles per wave and key tile
@@ -52,7 +59,7 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
   constexpr int LD = KT * CPR / NT;       // LDS-DMA pieces per thread and tile of K (and of V)
   constexpr int KSTEPS = D / 16, DT = D / 32;
   static_assert(KT * CPR % NT == 0 && LD >= 1);
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[ST * 2 * TILE_BYTES];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * TILE_BYTES];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -301,23 +308,17 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
     }
   };
   int buf = 0, i = i_begin;
-  auto fill = [&]() {
-#pragma unroll
-    for (int j = 0; j < ST - 1; ++j)
-      if (i_begin + j < i_end) stage(tile_at(i_begin + j), j);
-  };
-  auto arrive = [&](bool masked) {                      // tile i is there, the ST - 1 tiles behind it on their way
-    if (ST > 2 && i + ST - 2 < i_end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 2) * 2 * LD) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this wave's pieces of tile i have landed ...
+  auto arrive = [&](bool masked) {                      // tile i is there, tile i + 1 on its way
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // this wave's pieces of tile i have landed ...
     if (masked) clean(tile_at(i) * KT, buf);
-    __syncthreads();                                    // ... and everybody's; the slot of tile i - 1 has been read
-    if (i + ST - 1 < i_end) stage(tile_at(i + ST - 1), buf == 0 ? ST - 1 : buf - 1);
+    __syncthreads();                                    // ... and everybody's; the other slot has been read
+    if (i + 1 < i_end) stage(tile_at(i + 1), buf ^ 1);
   };
   auto on = [&]() {
     ++i;
-    buf = buf == ST - 1 ? 0 : buf + 1;
+    buf ^= 1;
   };
-  fill();
+  if (i_begin < i_end) stage(tile_at(i_begin), 0);
 #pragma unroll
   for (int ks = 0; ks < KSTEPS; ++ks) asm volatile("" ::"v"(qf[ks]));      // (there before the loop: its waits count DMAs alone)
   for (int stretch = 0; stretch < 3; ++stretch) {
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
     l_run = 0.f;
     buf = 0;
     i = i_begin;
-    fill();
+    if (i_begin < i_end) stage(tile_at(i_begin), 0);
     for (; i < i_end; on()) {
       arrive(true);
       const int base = tile_at(i) * KT + wk * KW;
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
   if constexpr (WK > 1) {
     // ---- the key waves' shares are merged through LDS by the first of them, register by register (the same rows lie in the same lanes)
     constexpr int R4 = DT * 4;                            // f32x4 per lane
-    static_assert((WK - 1) * WR * 64 * (R4 * 16 + 8) <= ST * 2 * TILE_BYTES);
+    static_assert((WK - 1) * WR * 64 * (R4 * 16 + 8) <= 4 * TILE_BYTES);
     f32x4* so = reinterpret_cast<f32x4*>(smem);
     float* sml = reinterpret_cast<float*>(smem + (WK - 1) * WR * R4 * 1024);
     __syncthreads();                                      // the last tile has been read
@@ -527,11 +528,11 @@ static WindowPlan window_plan(int64_t batch, int64_t sq, int64_t sk, int64_t kv_
   return w;
 }
 
-template <int D, int WR, int WK, int KW, int ST, int OCC>
+template <int D, int WR, int WK, int KW, int OCC>
 static int launch_window(const WindowParams& p, hipStream_t s) {
   const int64_t per_class = (int64_t)p.batch * p.kv_heads / p.classes * p.n_blocks * p.parts, xcds = 8 / p.classes;
   const int64_t grid = (per_class + xcds - 1) / xcds * 8;
-  attn_window_kernel<D, WR, WK, KW, ST, OCC><<<dim3((unsigned)grid), dim3(64 * WR * WK), 0, s>>>(p);
+  attn_window_kernel<D, WR, WK, KW, OCC><<<dim3((unsigned)grid), dim3(64 * WR * WK), 0, s>>>(p);
   FDM_CHECK_LAUNCH();
   return FDM_OK;
 }
@@ -565,7 +566,7 @@ int fdm_attn_window(void* o, const void* q, const void* k, const void* v, const 
   const int64_t group = q_heads / kv_heads;
   // places, rows and items are 32-bit numbers in the kernel (addresses are 64-bit)
   if (k_tok_stride > (1 << 22) || v_tok_stride > (1 << 22)) return FDM_ERR_UNSUPPORTED;      // (a tile's lane offsets are 32-bit)
-  if (sk > (1 << 30) || sq > (1 << 30) || sq * group > (1 << 30) || batch > (1 << 24)) return FDM_ERR_UNSUPPORTED;
+  if (sk > (1 << 29) || sq > (1 << 29) || sq * group > (1 << 30) || batch > (1 << 24)) return FDM_ERR_UNSUPPORTED;
   const int64_t win = window < sk ? window : (sk > 0 ? sk : 1), snk = sinks < sk ? sinks : sk;      // the same keys, and no overflow
   const WindowPlan w = window_plan(batch, sq, sk, kv_heads, group, head_dim, win, snk);
   const int64_t items = w.units * w.parts;
@@ -586,9 +587,9 @@ int fdm_attn_window(void* o, const void* q, const void* k, const void* v, const 
   hipStream_t s = to_stream(stream);
   int rc;
   if (head_dim == 128)
-    rc = w.form == 0 ? launch_window<128, 1, 1, 32, 2, 1>(p, s) : w.form == 1 ? launch_window<128, 4, 1, 64, 2, 2>(p, s) : w.form == 2 ? launch_window<128, 2, 2, 32, 2, 2>(p, s) : launch_window<128, 4, 2, 64, 2, 2>(p, s);
+    rc = w.form == 0 ? launch_window<128, 1, 1, 32, 1>(p, s) : w.form == 1 ? launch_window<128, 4, 1, 64, 2>(p, s) : w.form == 2 ? launch_window<128, 2, 2, 32, 2>(p, s) : launch_window<128, 4, 2, 64, 2>(p, s);
   else
-    rc = w.form == 0 ? launch_window<64, 1, 1, 32, 2, 2>(p, s) : w.form == 1 ? launch_window<64, 4, 1, 64, 2, 3>(p, s) : launch_window<64, 2, 2, 64, 2, 2>(p, s);
+    rc = w.form == 0 ? launch_window<64, 1, 1, 32, 2>(p, s) : w.form == 1 ? launch_window<64, 4, 1, 64, 3>(p, s) : launch_window<64, 2, 2, 64, 2>(p, s);
   if (rc != FDM_OK || w.parts == 1) return rc;
   return head_dim == 128 ? launch_merge<128>(p, w.rb_rows, s) : launch_merge<64>(p, w.rb_rows, s);
 }

@@ -115,7 +115,7 @@ def c_window(**kw):
 @pytest.mark.parametrize("kw,code", [(dict(o=None), -1), (dict(q=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(q=8200), -1), (dict(kts=63), -1), (dict(vbs=-512), -1),
                                      (dict(ql=2), -1), (dict(kl=6), -1), (dict(hq=3, hk=2), -1), (dict(hk=0), -1), (dict(window=0), -1), (dict(sinks=-1), -1),
                                      (dict(scale=0.0), -1), (dict(scale=-1.0), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(B=-1), -1),
-                                     (dict(D=96), -2), (dict(sk=1 << 31), -2), (dict(sq=1 << 31), -2), (dict(sq=0, q=None), 0), (dict(B=0, o=None), 0),
+                                     (dict(D=96), -2), (dict(sk=(1 << 29) + 1), -2), (dict(sq=(1 << 29) + 1), -2), (dict(sq=0, q=None), 0), (dict(B=0, o=None), 0),
                                      (dict(sq=1, sk=100000, window=100000), -1), (dict(sq=1, sk=100000, window=100000, ws=64, wsb=64), -1)])
 def test_window_attention_c_entry_refuses(kw, code):
     assert c_window(**kw) == code
