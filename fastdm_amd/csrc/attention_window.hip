@@ -30,6 +30,21 @@
 
 namespace fdm {
 
+// Division of 0 .. 2^31 - 1 by d, exact: i / d = (i * m) >> (32 + s) with s = ceil(log2 d) - 1 and m = ceil(2^(32 + s) / d), m < 2^32 (Granlund and Montgomery
+// 1994); m = 0: d is 1.  (A division by a kernel argument is 20 instructions in a row; the ten in front of a block's first load took 0.5 us.)
+struct Divider {
+  uint32_t m = 0, s = 0;
+  int d = 1;
+  Divider() = default;
+  __host__ explicit Divider(int64_t by) : d((int)by) {
+    if (by <= 1) return;
+    while (((int64_t)2 << s) < by) ++s;
+    m = (uint32_t)((((uint64_t)1 << (32 + s)) + by - 1) / by);
+  }
+  __device__ __forceinline__ int operator()(int i) const { return m ? (int)(__umulhi((uint32_t)i, m) >> s) : i; }
+  __device__ __forceinline__ int rest(int i) const { return i - (*this)(i) * d; }
+};
+
 struct WindowParams {
   bf16_t* o;
   const bf16_t* q;
@@ -42,7 +57,8 @@ struct WindowParams {
   int window, sinks;
   int n_blocks;         // row blocks of a (batch, kv head)
   int parts;            // parts a block's tile list is cut into
-  int classes;          // of (batch, kv head) pairs, one or more XCDs each: 1, 2, 4 or 8
+  int classes_log2;     // of (batch, kv head) pairs, one or more XCDs each: 1, 2, 4 or 8 classes
+  Divider by_group, by_parts, by_class_pairs, by_kv_heads;
   float scale_log2e;
   float* ws_o;          // parts > 1: [batch * kv_heads * n_blocks][parts][rows of a block][D], unnormalised
   float* ws_ml;         // ... [..][..][rows][2]: maximum (exp2 domain), sum
@@ -69,14 +85,14 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
   // The blocks that run at one time on an XCD share its L2: a class of (batch, kv head) pairs belongs to 8 / classes XCDs (classes: the largest
   // divisor of 8 that deals the pairs out evenly), and their row blocks are taken from the last, longest lists to the first, pair by pair.
   // Against runs of consecutive row blocks per XCD: 16384 tokens, window 4096, 8 pairs 1060 -> 944 us; open window 2664 -> 1979 us.
-  const int per = p.batch * p.kv_heads / p.classes;
-  const int it = (blockIdx.x >> 3) * (8 / p.classes) + (blockIdx.x & 7) / p.classes;
-  const int part = it % p.parts;
-  const int rb = p.n_blocks - 1 - it / p.parts / per;
-  const int bk = (blockIdx.x & 7) % p.classes + p.classes * (it / p.parts % per);
+  const int xcd = blockIdx.x & 7, lg = p.classes_log2;
+  const int it = ((int)(blockIdx.x >> 3) << (3 - lg)) + (xcd >> lg);
+  const int u = p.by_parts(it), part = it - u * p.parts;
+  const int rb = p.n_blocks - 1 - p.by_class_pairs(u);
+  const int bk = (xcd & ((1 << lg) - 1)) + (p.by_class_pairs.rest(u) << lg);
   if (rb < 0) return;
   const int unit = bk * p.n_blocks + rb;
-  const int b = bk / p.kv_heads, kvh = bk % p.kv_heads;
+  const int b = p.by_kv_heads(bk), kvh = bk - b * p.kv_heads;
   const int G = p.group;
 
   int q_len = p.sq, kv_len = p.sk;
@@ -90,10 +106,10 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
   const int n_rows = p.sq * G;
   const int row = rb * RB + wr * 32 + lq;
   const int rowc = min(row, n_rows - 1);
-  const int tok = rowc / G, head = kvh * G + rowc % G;
+  const int tok = p.by_group(rowc), head = kvh * G + rowc - tok * G;
   const bool live = row < n_rows && tok < q_len;
-  const int wt_lo = (rb * RB + wr * 32) / G, wt_hi = min(min(rb * RB + wr * 32 + 31, n_rows - 1) / G, q_len - 1);
-  const int bt_lo = rb * RB / G, bt_hi = min(min(rb * RB + RB - 1, n_rows - 1) / G, q_len - 1);
+  const int wt_lo = p.by_group(rb * RB + wr * 32), wt_hi = min(p.by_group(min(rb * RB + wr * 32 + 31, n_rows - 1)), q_len - 1);
+  const int bt_lo = p.by_group(rb * RB), bt_hi = min(p.by_group(min(rb * RB + RB - 1, n_rows - 1)), q_len - 1);
   const int wp_lo = first + wt_lo, wp_hi = first + wt_hi;        // wt_lo > wt_hi: the wave has no row
   const int place = first + tok;
 
@@ -108,7 +124,7 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
     w_begin = min(w_begin, w_end);
   }
   const int n_list = n_sink + w_end - w_begin;
-  const int i_begin = (int)((int64_t)part * n_list / p.parts), i_end = (int)((int64_t)(part + 1) * n_list / p.parts);
+  const int i_begin = p.by_parts(part * n_list), i_end = p.by_parts((part + 1) * n_list);      // (at most 64 parts of lists of 2^24 tiles)
   auto tile_at = [&](int i) { return i < n_sink ? i : i - n_sink + w_begin; };
 
   const bf16_t* kbase = p.k + (int64_t)b * p.k_bs + (int64_t)kvh * D;
@@ -530,7 +546,7 @@ static WindowPlan window_plan(int64_t batch, int64_t sq, int64_t sk, int64_t kv_
 
 template <int D, int WR, int WK, int KW, int OCC>
 static int launch_window(const WindowParams& p, hipStream_t s) {
-  const int64_t per_class = (int64_t)p.batch * p.kv_heads / p.classes * p.n_blocks * p.parts, xcds = 8 / p.classes;
+  const int64_t per_class = (((int64_t)p.batch * p.kv_heads) >> p.classes_log2) * p.n_blocks * p.parts, xcds = 8 >> p.classes_log2;
   const int64_t grid = (per_class + xcds - 1) / xcds * 8;
   attn_window_kernel<D, WR, WK, KW, OCC><<<dim3((unsigned)grid), dim3(64 * WR * WK), 0, s>>>(p);
   FDM_CHECK_LAUNCH();
@@ -580,7 +596,11 @@ int fdm_attn_window(void* o, const void* q, const void* k, const void* v, const 
   p.batch = (int)batch; p.sq = (int)sq; p.sk = (int)sk; p.kv_heads = kv_heads; p.group = (int)group;
   p.window = (int)win; p.sinks = (int)snk; p.n_blocks = (int)w.n_blocks; p.parts = w.parts;
   const int64_t pairs = batch * kv_heads;
-  p.classes = pairs % 8 == 0 ? 8 : pairs % 4 == 0 ? 4 : pairs % 2 == 0 ? 2 : 1;
+  p.classes_log2 = pairs % 8 == 0 ? 3 : pairs % 4 == 0 ? 2 : pairs % 2 == 0 ? 1 : 0;
+  p.by_group = Divider(group);
+  p.by_parts = Divider(w.parts);
+  p.by_class_pairs = Divider(pairs >> p.classes_log2);
+  p.by_kv_heads = Divider(kv_heads);
   p.scale_log2e = scale * 1.4426950408889634f;
   p.ws_o = (float*)workspace;
   p.ws_ml = p.ws_o + w.units * w.parts * w.rb_rows * head_dim;
