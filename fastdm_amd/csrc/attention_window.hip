@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
 
   // ---- K / V staging by LDS-DMA: lane-linear destination, the swizzle is applied to the source.  A piece is a wave-uniform tile base plus a 32-bit
   //      lane offset that stays.  The DMA is an asm statement (it writes no register): hipcc puts s_waitcnt vmcnt(0) in front of LDS reads that
-  //      follow its builtin, which is the next tile's DMA here; the waits are the two lines at the top of the loop.
+  //      follow its builtin, which is the next tile's DMA here; the waits are the two lines at the top of the loop.  Inside: one wait state between m0 and
+  //      its use, five between a base that the vector unit may have written and the address.
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem + wave * 1024;
   uint32_t kofs[LD], vofs[LD];
 #pragma unroll
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
     vofs[i] = (uint32_t)(r * (int)p.v_ts * 2 + Swz<D>::v(r, slot % CPR) * 16);
   }
   auto dma = [&](const bf16_t* base, uint32_t ofs, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(ofs), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(ofs), "s"(base) : "memory");
   };
   auto stage = [&](int t, int buf) {
     const uint32_t lds = lds0 + buf * 2 * TILE_BYTES;
