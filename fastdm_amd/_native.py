@@ -339,6 +339,38 @@ def row_stride(t, what):
     return stride
 
 
+def crosses(a, out, same=False):
+    """Whether `out` [.., rows, width], being written, lies across `a`: rows (dense, at any strides) that share memory.  The very same rows are in place
+    and do not count, unless `same`.  Rows of equal strides may lie between each other's (slices of one tensor); of different strides, any common
+    stretch counts."""
+    if 0 in a.shape or out.shape[-1] == 0:
+        return False
+    if a is out:
+        return same
+    axes = [d for d in range(a.ndim - 1) if a.shape[d] > 1]
+    sa, so = [a.stride(d) for d in axes], [out.stride(d) for d in axes]
+    pa, po, size = a.data_ptr(), out.data_ptr(), a.element_size()
+    if pa == po and sa == so:
+        return same or a.shape != out.shape
+    wa, wo, steps = a.shape[-1], out.shape[-1], [a.shape[d] - 1 for d in axes]
+    apart = (po - pa) // size
+    if apart >= wa + sum(n * s for n, s in zip(steps, sa)) or -apart >= wo + sum(n * s for n, s in zip(steps, so)):
+        return False
+    return sa != so or _meet(apart, wa, wo, sorted(zip(sa, steps)))
+
+
+def _meet(apart, wa, wo, axes):
+    """Whether [apart + sum n_i s_i, .. + wo) and [0, wa) share a number for whole n_i, |n_i| <= the axis' steps; axes: (s_i, steps), the widest last."""
+    if not axes:
+        return -wo < apart < wa
+    *rest, (s, steps) = axes
+    if s == 0:
+        return _meet(apart, wa, wo, rest)
+    reach = sum(t * n for t, n in rest)
+    low, high = max(-((apart + wo - 1 + reach) // s), -steps), min((wa - 1 + reach - apart) // s, steps)
+    return any(_meet(apart + n * s, wa, wo, rest) for n in range(low, high + 1))
+
+
 _raw_stream = None
 
 

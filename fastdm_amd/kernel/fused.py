@@ -95,7 +95,7 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     """h = x + residual (kept in bf16); y = h / rms(h) * weight, as bf16 (quant=None) or quantised per row for the next W8A8 linear -- one pass
     where an addition, rms_norm and quantize_rows take three, and ONE rounding of y (it is not rounded to bf16 on its way to 8 bits).
     x, residual: [rows, width] bf16, rows may be column slices of wider matrices.  Returns (bf16 y | None, Quantized | None, h | None) like ln_modulate.
-    residual_out: where h goes (may be `residual` or `x` itself: in place).  residual=None: the norm of x alone, h is None.
+    residual_out: where h goes (may be `residual` or `x` itself: in place; not across either of them).  residual=None: the norm of x alone, h is None.
     e4m3: scale = max|y| / 448; int8: asymmetric (scale, azp), as the row quantisers."""
     gpu = N.gpu_of("add_rms_norm", x, residual, weight, residual_out)
     assert x.ndim == 2 and x.dtype == BF16 and weight.dtype == BF16, "add_rms_norm: x [rows, width] and weight in bf16"
@@ -113,6 +113,7 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
         else:
             assert residual_out.shape == shape and residual_out.dtype == BF16, "add_rms_norm: residual_out as x"
             hs = N.row_stride(residual_out, "add_rms_norm")
+            assert not (N.crosses(x, residual_out) or N.crosses(residual, residual_out)), "add_rms_norm: residual_out lies across x or residual"
         residual_ptr, h_ptr = residual.data_ptr(), residual_out.data_ptr()
     else:
         assert residual_out is None, "add_rms_norm: residual_out without residual"

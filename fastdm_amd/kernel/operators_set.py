@@ -64,7 +64,6 @@ def _rotary_side(x, out, B, S, head_size, what):
     o_bs, o_ts, o_es = out.stride()
     assert o_es == 1, f"rotary_positions: {what}_out's tokens must be dense"
     assert (S <= 1 or o_ts >= width) and (B <= 1 or o_bs >= width), f"rotary_positions: {what}_out overlaps itself"
-    assert out.data_ptr() != x.data_ptr() or (x_bs, x_ts) == (o_bs, o_ts), f"rotary_positions: {what} in place needs the same strides"
     return out, width // head_size, x_bs, x_ts, o_bs, o_ts
 
 
@@ -76,12 +75,13 @@ def rotary_positions(query: torch.Tensor, key: Optional[torch.Tensor], head_size
     contexts).  Next to rotary_pos_embedding, which reads a bf16 cos | sin table of positions 0 .. S - 1: here the angle is taken in 64 bits at any
     place and the result is rounded once.  is_neox: pairs (i, i + rotary_dim / 2) instead of (2i, 2i + 1).  Inputs may be slices of a fused
     projection (any batch and token strides); returns (query_out, key_out), new tensors unless given -- `query` / `key` themselves for in place,
-    a cache's slice for a key that is stored there."""
+    a cache's slice for a key that is stored there; an output that lies across an input otherwise is refused."""
     gpu = N.gpu_of("rotary_positions", query, key, positions, query_out, key_out, frequencies.turns)
     rot = frequencies.rotary_dim
     assert rot <= head_size, "rotary_positions: rotary_dim is larger than the head"
     assert query.ndim == 3, "rotary_positions: query [B, S, heads * head_size]"
     B, S, _ = query.shape
+    q_given, k_given = query_out is not None, key_out is not None
     query_out, q_heads, *q_strides = _rotary_side(query, query_out, B, S, head_size, "query")
     k_heads = key_ptr = key_out_ptr = 0
     k_strides = (0, 0, 0, 0)
@@ -90,6 +90,11 @@ def rotary_positions(query: torch.Tensor, key: Optional[torch.Tensor], head_size
         key_ptr, key_out_ptr = key.data_ptr(), key_out.data_ptr()
     else:
         assert key_out is None, "rotary_positions: key_out without key"
+    if q_given:
+        assert not (N.crosses(query, query_out) or key is not None and N.crosses(key, query_out, same=True)), "rotary_positions: query_out lies across an input"
+    if k_given:
+        assert not (N.crosses(key, key_out) or N.crosses(query, key_out, same=True) or N.crosses(query_out, key_out, same=True)), \
+            "rotary_positions: key_out lies across an input or query_out"
     p_ptr = p_bs = p_ts = p_bytes = 0
     if positions is not None:
         assert positions.dtype in (torch.int32, torch.int64), "rotary_positions: positions int32 or int64"

@@ -446,9 +446,9 @@ int fdm_qk_norm_rope_inplace(void* qkv, const void* wq, const void* wk, const vo
  *   quant_mode 0: out_bf16 = bf16(y);  1: out_scale = max(max|y|, 1e-12) / 448, out_q = e4m3(y / out_scale);
  *   quant_mode 2: out_scale = (max y - min y) / 255, out_azp = -128 - rint(min y / out_scale), out_q = rint(y / out_scale) + out_azp (the spread
  *   counts as at least max|y| / 16 and 1e-12: a row of one value stays representable).
- * x, res, h_out: [rows, width] bf16 with their own row strides (elements); outputs compact.  h_out may be x or res.  Any width <= 65536 and any
- * (element) alignment; multiples of 8 on 16-byte aligned rows take whole vectors.  A row with a NaN or an infinity gives NaNs (its 8-bit rows: a NaN
- * scale).  rows <= 2^31 - 1.                                                                                                          */
+ * x, res, h_out: [rows, width] bf16 with their own row strides (elements); outputs compact.  h_out may be x or res (not other rows of theirs).  Any
+ * width <= 65536 and any (element) alignment; multiples of 8 on 16-byte aligned rows take whole vectors.  A row with a NaN or an infinity gives NaNs
+ * (its 8-bit rows: a NaN scale); a row whose sum of squares passes fp32's range gives zeros.  rows <= 2^31 - 1.                            */
 int fdm_add_rms_norm(void* out_bf16, void* out_q, float* out_scale, int32_t* out_azp, int quant_mode, const void* x, const void* res,
                      const void* weight, void* h_out, int64_t rows, int64_t width, int64_t x_row_stride, int64_t res_row_stride,
                      int64_t h_row_stride, float eps, fdm_stream_t stream);
@@ -471,7 +471,8 @@ int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, c
  *   q_lens, kv_lens: int32 [batch] on the device, or NULL for sq / sk (values outside 0 .. sq / sk count as the nearest).  The queries of a sequence are
  *   the last q_len of its kv_len tokens: row t < q_len is at place kv_len - q_len + t and sees key j iff j <= place and (place - j < window or j < sinks).
  *   Rows at or past q_len, and rows that see nothing, are zeros.  Keys at or past kv_len are not read; what a row does not see does not reach it, NaNs
- *   and infinities included.  softmax(q k^T * scale) v with fp32 statistics, scale > 0; window >= 1 (>= sk: plain causal), sinks >= 0; sk, sq <= 2^29.
+ *   and infinities included; where a row sees one in v, its result is not finite (NaN also for an infinity).
+ *   softmax(q k^T * scale) v with fp32 statistics, scale > 0; window >= 1 (>= sk: plain causal), sinks >= 0; sk, sq <= 2^29.
  * workspace: 16-byte aligned, >= fdm_attn_window_workspace_bytes(...) of the same arguments (0: none), rewritten by every call.                */
 int64_t fdm_attn_window_workspace_bytes(int64_t batch, int64_t sq, int64_t sk, int q_heads, int kv_heads, int head_dim, int64_t window, int64_t sinks);
 int fdm_attn_window(void* o, const void* q, const void* k, const void* v, const int32_t* q_lens, const int32_t* kv_lens, int64_t batch, int64_t sq,

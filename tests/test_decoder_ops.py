@@ -167,3 +167,34 @@ def test_launch_goes_to_the_tensors_device(monkeypatch):
     assert seen == [(0, (1, 100)), (3, (2, 103))] and current[0] == 0
     with pytest.raises(RuntimeError, match="x failed: unsupported"):
         N.launch("x", 0, lambda *a: -2)
+
+
+def test_outputs_across_inputs_are_told_from_slices_and_from_in_place():
+    m = torch.zeros(8, 96, dtype=BF16)
+    a = m[:4, :32]
+    assert not N.crosses(a, m[:4, :32]) and N.crosses(a, m[:4, :32], same=True) and not N.crosses(a, a) and N.crosses(a, a, same=True)      # in place
+    assert not N.crosses(a, m[:4, 32:64]) and not N.crosses(a, m[1:5, 32:64]) and not N.crosses(a, m[4:, :32])                              # beside, behind
+    assert N.crosses(a, m[1:5, :32]) and N.crosses(m[1:5, :32], a) and N.crosses(a, m[:4, 16:48]) and N.crosses(m[:4, 16:48], a)            # shifted
+    assert N.crosses(a, m.view(-1)[:256].view(4, 64)[:, :32]) and not N.crosses(a, torch.zeros(4, 32, dtype=BF16))                         # other strides
+    assert N.crosses(m[:1, :32], m[:1, 16:48]) and not N.crosses(m[:1, :32], m[:1, 32:64]) and not N.crosses(m[:0], m[:0], same=True)              # one row, none
+    b = torch.zeros(2, 6, 96, dtype=BF16)
+    assert not N.crosses(b[..., :64], b[..., 64:], same=True) and N.crosses(b[..., :64], b[..., 32:]) and N.crosses(b[:, :5, :64], b[:, 1:, :64])
+    assert not N.crosses(b[:, :3, :64], b[:, 3:, 64:]) and not N.crosses(b[:1, :, :64], b[1:, :, :64])
+    assert not N.crosses(b[:, :3, :64], b[:, 3:, :64], same=True) and N.crosses(b[:, :4, :64], b[:, 2:, :64])       # tokens in front of others'
+
+
+def test_outputs_across_inputs_against_every_row():
+    """All pairs of slices of a small tensor, against the addresses themselves."""
+    import itertools
+    base = torch.zeros(3, 4, 6, dtype=BF16)
+    places = torch.arange(base.numel()).view(3, 4, 6)
+    cuts = [(slice(i, i + B), slice(j, j + S), slice(c, c + W)) for B, S, W in ((2, 2, 3), (1, 3, 2), (2, 1, 4), (1, 1, 6))
+            for i in range(4 - B) for j in range(5 - S) for c in range(7 - W)]
+    for x, y in itertools.product(cuts, cuts):
+        a, out = base[x], base[y]
+        if a.shape[:2] == out.shape[:2]:
+            share = bool(set(places[x].flatten().tolist()) & set(places[y].flatten().tolist()))
+            assert N.crosses(a, out, same=True) == share, (x, y)
+            assert N.crosses(a, out) == (share and x != y), (x, y)
+    other = base.view(4, 3, 6)
+    assert N.crosses(base[:2, :2], other[:2, :2]) and not N.crosses(base[:1, :2], other[3:, :2])

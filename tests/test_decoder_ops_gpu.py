@@ -658,3 +658,21 @@ def test_rotary_positions_refusals(what):
             "key out without key": lambda: rotary_positions(q, None, 64, f, key_out=q)}[what]
     with pytest.raises((AssertionError, RuntimeError)):
         call()
+
+
+@pytest.mark.parametrize("what", ["next rows", "next columns", "other strides", "query_out on key", "key_out on query", "key_out on query_out", "query_out a token on"])
+def test_outputs_across_inputs_are_refused(what):
+    from fastdm_amd.kernel.fused import add_rms_norm
+    from fastdm_amd.kernel.operators_set import rotary_positions
+    from fastdm_amd.layer.embeddings import RotaryFrequencies
+    m, w, f = randn(gen(1), 8, 128), torch.ones(64, device="cuda", dtype=BF16), RotaryFrequencies(64, device="cuda")
+    kept = m.clone()
+    x, r, t = m[:4, :64], randn(gen(2), 4, 64), m[None]
+    q, k, o = t[:, :6, :64], t[:, :6, 64:], randn(gen(3), 1, 6, 64)
+    call = {"next rows": lambda: add_rms_norm(x, r, w, 1e-6, residual_out=m[1:5, :64]), "next columns": lambda: add_rms_norm(r, x, w, 1e-6, residual_out=m[:4, 32:96]),
+            "other strides": lambda: add_rms_norm(x, r, w, 1e-6, residual_out=m.view(16, 64)[:4]),
+            "query_out on key": lambda: rotary_positions(q, k, 64, f, query_out=k), "key_out on query": lambda: rotary_positions(q, k, 64, f, query_out=o, key_out=q),
+            "key_out on query_out": lambda: rotary_positions(q, k, 64, f, query_out=o, key_out=o), "query_out a token on": lambda: rotary_positions(q, k, 64, f, query_out=t[:, 1:7, :64])}[what]
+    with pytest.raises(AssertionError):
+        call()
+    assert torch.equal(m, kept)
