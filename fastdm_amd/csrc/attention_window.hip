@@ -27,6 +27,7 @@
 #include <type_traits>
 #include "common.h"
 #include "attn_common.h"
+#include "launch.h"
 
 namespace fdm {
 
@@ -57,6 +58,7 @@ struct WindowParams {
   int window, sinks;
   int n_blocks;         // row blocks of a (batch, kv head)
   int parts;            // parts a block's tile list is cut into
+  int block0;           // of this launch, a multiple of 8
   int classes_log2;     // of (batch, kv head) pairs, one or more XCDs each: 1, 2, 4 or 8 classes
   Divider by_group, by_parts, by_class_pairs, by_kv_heads;
   float scale_log2e;
@@ -85,8 +87,8 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
   // The blocks that run at one time on an XCD share its L2: a class of (batch, kv head) pairs belongs to 8 / classes XCDs (classes: the largest
   // divisor of 8 that deals the pairs out evenly), and their row blocks are taken from the last, longest lists to the first, pair by pair.
   // Against runs of consecutive row blocks per XCD: 16384 tokens, window 4096, 8 pairs 1060 -> 944 us; open window 2664 -> 1979 us.
-  const int xcd = blockIdx.x & 7, lg = p.classes_log2;
-  const int it = ((int)(blockIdx.x >> 3) << (3 - lg)) + (xcd >> lg);
+  const int block = p.block0 + (int)blockIdx.x, xcd = block & 7, lg = p.classes_log2;
+  const int it = ((block >> 3) << (3 - lg)) + (xcd >> lg);
   const int u = p.by_parts(it), part = it - u * p.parts;
   const int rb = p.n_blocks - 1 - p.by_class_pairs(u);
   const int bk = (xcd & ((1 << lg) - 1)) + (p.by_class_pairs.rest(u) << lg);
@@ -493,7 +495,7 @@ __global__ void __launch_bounds__(256) attn_window_merge_kernel(const WindowPara
 
 template <int D>
 static int launch_merge(const WindowParams& p, int rb_rows, hipStream_t s) {
-  const int64_t rows = (int64_t)p.batch * p.kv_heads * p.sq * p.group;
+  const int64_t rows = (int64_t)p.batch * p.kv_heads * p.sq * p.group;      // (parts: fewer units than places on the chip, so one launch holds them)
   if (p.parts > 4) {
     constexpr int PG = 256 / (D / 4);
     attn_window_merge_kernel<D, PG><<<dim3((unsigned)rows), dim3(256), 0, s>>>(p, rb_rows);
@@ -546,12 +548,15 @@ static WindowPlan window_plan(int64_t batch, int64_t sq, int64_t sk, int64_t kv_
 }
 
 template <int D, int WR, int WK, int KW, int OCC>
-static int launch_window(const WindowParams& p, hipStream_t s) {
+static int launch_window(WindowParams p, hipStream_t s) {
   const int64_t per_class = (((int64_t)p.batch * p.kv_heads) >> p.classes_log2) * p.n_blocks * p.parts, xcds = 8 >> p.classes_log2;
   const int64_t grid = (per_class + xcds - 1) / xcds * 8;
-  attn_window_kernel<D, WR, WK, KW, OCC><<<dim3((unsigned)grid), dim3(64 * WR * WK), 0, s>>>(p);
-  FDM_CHECK_LAUNCH();
-  return FDM_OK;
+  return launch_pieces(grid, 64 * WR * WK, [&](int64_t first, unsigned count) -> int {
+    p.block0 = (int)first;
+    attn_window_kernel<D, WR, WK, KW, OCC><<<dim3(count), dim3(64 * WR * WK), 0, s>>>(p);
+    FDM_CHECK_LAUNCH();
+    return FDM_OK;
+  });
 }
 
 }  // namespace fdm

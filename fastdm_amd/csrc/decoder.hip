@@ -1,6 +1,7 @@
 // Row kernels of a decoder layer: residual addition + RMS norm with a bf16 or 8-bit output, and rotary positions at given places.
 // HBM-bound like the rows kernels of elementwise.hip: 16-byte vectors per lane, every byte read and written once.
 #include "common.h"
+#include "launch.h"
 
 namespace fdm {
 
@@ -27,6 +28,7 @@ struct NormArgs {
   const bf16_t* res;
   const bf16_t* w;
   int64_t x_stride, res_stride, h_stride;
+  int64_t row0;         // of this launch
   int width;
   float eps;
 };
@@ -36,7 +38,7 @@ template <int THREADS, int NIT, int MODE, bool RES, bool EDGE>
 __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(const NormArgs p) {
   constexpr int NW = THREADS / 64;
   __shared__ float red[3][NW];
-  const int64_t row = blockIdx.x;
+  const int64_t row = p.row0 + blockIdx.x;
   const int tid = threadIdx.x;
   const int nvec = (p.width + 7) >> 3;
   const bf16_t* xr = p.x + row * p.x_stride;
@@ -185,16 +187,21 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(const NormArgs p)
 }
 
 template <int THREADS, int NIT>
-static void launch_norm(const NormArgs& a, int64_t rows, int mode, bool edge, hipStream_t s) {
-#define FDM_NORM(M, R, E) add_rms_norm_kernel<THREADS, NIT, M, R, E><<<dim3((unsigned)rows), dim3(THREADS), 0, s>>>(a)
+static int launch_norm(NormArgs a, int64_t rows, int mode, bool edge, hipStream_t s) {
+#define FDM_NORM(M, R, E) add_rms_norm_kernel<THREADS, NIT, M, R, E><<<dim3(count), dim3(THREADS), 0, s>>>(a)
 #define FDM_NORM_M(M)                                                   \
   if (a.res) { if (edge) FDM_NORM(M, true, true); else FDM_NORM(M, true, false); } \
   else { if (edge) FDM_NORM(M, false, true); else FDM_NORM(M, false, false); }
-  switch (mode) {
-    case 0: FDM_NORM_M(0); break;
-    case 1: FDM_NORM_M(1); break;
-    default: FDM_NORM_M(2); break;
-  }
+  return launch_pieces(rows, THREADS, [&](int64_t first, unsigned count) -> int {
+    a.row0 = first;
+    switch (mode) {
+      case 0: FDM_NORM_M(0); break;
+      case 1: FDM_NORM_M(1); break;
+      default: FDM_NORM_M(2); break;
+    }
+    FDM_CHECK_LAUNCH();
+    return FDM_OK;
+  });
 #undef FDM_NORM_M
 #undef FDM_NORM
 }
@@ -216,6 +223,7 @@ struct RopeAtArgs {
   int64_t pos_bs, pos_ts; // strides in elements
   int64_t q_bs, q_ts, k_bs, k_ts, qo_bs, qo_ts, ko_bs, ko_ts;
   int64_t tokens;
+  int64_t block0;         // of this launch
   int seq, q_heads, k_heads, head, rot;
   int pos_bytes;          // 4 or 8
   int items;              // work items per token
@@ -266,7 +274,7 @@ __global__ void __launch_bounds__(256) rope_at_kernel(const RopeAtArgs p) {
   extern __shared__ float2 turn_cs[];            // [tok_per_block][rot / 2]
   __shared__ int64_t at_q[ROPE_MAX_TOK], at_k[ROPE_MAX_TOK], at_qo[ROPE_MAX_TOK], at_ko[ROPE_MAX_TOK];
   const int half = p.rot >> 1;
-  const int64_t tok0 = (int64_t)blockIdx.x * p.tok_per_block;
+  const int64_t tok0 = (p.block0 + blockIdx.x) * p.tok_per_block;
   const int ntok = (int)min((int64_t)p.tok_per_block, p.tokens - tok0);
 
   if (threadIdx.x < ntok) {
@@ -371,19 +379,17 @@ int fdm_add_rms_norm(void* out_bf16, void* out_q, float* out_scale, int32_t* out
   const bool edge = (width & 7) || (at & 15) || (reinterpret_cast<uintptr_t>(out_q) & 7) || (x_row_stride & 7) ||
                     (res && ((res_row_stride & 7) || (h_row_stride & 7)));
   const NormArgs a{(bf16_t*)out_bf16, (uint8_t*)out_q, out_scale, out_azp, (bf16_t*)h_out, (const bf16_t*)x, (const bf16_t*)res,
-                   (const bf16_t*)weight, x_row_stride, res_row_stride, h_row_stride, (int)width, eps};
+                   (const bf16_t*)weight, x_row_stride, res_row_stride, h_row_stride, 0, (int)width, eps};
   hipStream_t s = to_stream(stream);
   const int nvec = (int)((width + 7) >> 3);
-  if (nvec <= 64) launch_norm<64, 1>(a, rows, quant_mode, edge, s);
-  else if (nvec <= 256) launch_norm<256, 1>(a, rows, quant_mode, edge, s);
-  else if (nvec <= 512) launch_norm<256, 2>(a, rows, quant_mode, edge, s);
-  else if (nvec <= 768) launch_norm<256, 3>(a, rows, quant_mode, edge, s);
-  else if (nvec <= 1024) launch_norm<512, 2>(a, rows, quant_mode, edge, s);
-  else if (nvec <= 2048) launch_norm<512, 4>(a, rows, quant_mode, edge, s);
-  else if (nvec <= 4096) launch_norm<1024, 4>(a, rows, quant_mode, edge, s);
-  else launch_norm<1024, 8>(a, rows, quant_mode, edge, s);
-  FDM_CHECK_LAUNCH();
-  return FDM_OK;
+  if (nvec <= 64) return launch_norm<64, 1>(a, rows, quant_mode, edge, s);
+  if (nvec <= 256) return launch_norm<256, 1>(a, rows, quant_mode, edge, s);
+  if (nvec <= 512) return launch_norm<256, 2>(a, rows, quant_mode, edge, s);
+  if (nvec <= 768) return launch_norm<256, 3>(a, rows, quant_mode, edge, s);
+  if (nvec <= 1024) return launch_norm<512, 2>(a, rows, quant_mode, edge, s);
+  if (nvec <= 2048) return launch_norm<512, 4>(a, rows, quant_mode, edge, s);
+  if (nvec <= 4096) return launch_norm<1024, 4>(a, rows, quant_mode, edge, s);
+  return launch_norm<1024, 8>(a, rows, quant_mode, edge, s);
 }
 
 int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, const void* turns, const void* positions, int position_bytes,
@@ -441,17 +447,20 @@ int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, c
   const size_t lds = (size_t)tok * half * sizeof(float2);
   hipStream_t s = to_stream(stream);
 #define FDM_ROPE_AT(V)                                                                              \
-  if (is_neox) rope_at_kernel<V, true><<<dim3((unsigned)grid), dim3(256), lds, s>>>(a);             \
-  else rope_at_kernel<V, false><<<dim3((unsigned)grid), dim3(256), lds, s>>>(a)
-  switch (v) {
-    case 8: FDM_ROPE_AT(8); break;
-    case 4: FDM_ROPE_AT(4); break;
-    case 2: FDM_ROPE_AT(2); break;
-    default: FDM_ROPE_AT(1); break;
-  }
+  if (is_neox) rope_at_kernel<V, true><<<dim3(count), dim3(256), lds, s>>>(a);                      \
+  else rope_at_kernel<V, false><<<dim3(count), dim3(256), lds, s>>>(a)
+  return launch_pieces(grid, 256, [&](int64_t first, unsigned count) -> int {
+    a.block0 = first;
+    switch (v) {
+      case 8: FDM_ROPE_AT(8); break;
+      case 4: FDM_ROPE_AT(4); break;
+      case 2: FDM_ROPE_AT(2); break;
+      default: FDM_ROPE_AT(1); break;
+    }
+    FDM_CHECK_LAUNCH();
+    return FDM_OK;
+  });
 #undef FDM_ROPE_AT
-  FDM_CHECK_LAUNCH();
-  return FDM_OK;
 }
 
 }  // extern "C"

@@ -448,7 +448,8 @@ int fdm_qk_norm_rope_inplace(void* qkv, const void* wq, const void* wk, const vo
  *   counts as at least max|y| / 16 and 1e-12: a row of one value stays representable).
  * x, res, h_out: [rows, width] bf16 with their own row strides (elements); outputs compact.  h_out may be x or res (not other rows of theirs).  Any
  * width <= 65536 and any (element) alignment; multiples of 8 on 16-byte aligned rows take whole vectors.  A row with a NaN or an infinity gives NaNs
- * (its 8-bit rows: a NaN scale); a row whose sum of squares passes fp32's range gives zeros.  rows <= 2^31 - 1.                            */
+ * (its 8-bit rows: a NaN scale); a row whose sum of squares passes fp32's range gives zeros.  rows <= 2^31 - 1 (in several launches where one does not
+ * hold the threads; so the other two entries).                                                                                              */
 int fdm_add_rms_norm(void* out_bf16, void* out_q, float* out_scale, int32_t* out_azp, int quant_mode, const void* x, const void* res,
                      const void* weight, void* h_out, int64_t rows, int64_t width, int64_t x_row_stride, int64_t res_row_stride,
                      int64_t h_row_stride, float eps, fdm_stream_t stream);

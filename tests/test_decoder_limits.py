@@ -1,0 +1,45 @@
+"""CPU: the decoder-side operators at and past the sizes they can take."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fastdm_amd", "csrc")
+
+
+def test_huge_grids_go_in_pieces_that_a_launch_can_hold(tmp_path):
+    """launch_pieces: under 2^32 threads each, the blocks in order and each once, first blocks multiples of 8; ends with the first failure."""
+    compiler = shutil.which("g++")
+    if compiler is None:
+        pytest.skip("needs a C++ compiler")
+    source = tmp_path / "pieces.cpp"
+    source.write_text("""
+#include "launch.h"
+#include <cstdio>
+#include <initializer_list>
+int main() {
+  const int64_t blocks[] = {0, 1, 7, 8, 9, 67108855, 67108856, 67108857, (int64_t)1 << 24, ((int64_t)1 << 24) + 1, ((int64_t)1 << 26) + 3, 0x7fffffff};
+  for (int threads : {64, 128, 256, 512, 1024})
+    for (int64_t n : blocks) {
+      int64_t next = 0, pieces = 0;
+      bool ok = true;
+      const int rc = fdm::launch_pieces(n, threads, [&](int64_t first, unsigned count) {
+        ok = ok && first == next && first % 8 == 0 && count > 0 && (uint64_t)count * threads < ((uint64_t)1 << 32);
+        next = first + count;
+        ++pieces;
+        return 0;
+      });
+      const int64_t fewest = (n * threads + 0xffffffffLL) >> 32;
+      ok = ok && rc == 0 && next == n && pieces >= fewest && pieces <= fewest + 1 && (n * threads > 0xfffff000LL || pieces == (n > 0));
+      int calls = 0;
+      ok = ok && (n == 0 || (fdm::launch_pieces(n, threads, [&](int64_t, unsigned) { ++calls; return -3; }) == -3 && calls == 1));
+      if (!ok) { printf("%lld blocks of %d\\n", (long long)n, threads); return 1; }
+    }
+  return 0;
+}
+""")
+    binary = str(tmp_path / "pieces")
+    subprocess.run([compiler, "-std=c++17", "-O1", "-I", CSRC, str(source), "-o", binary], check=True)
+    done = subprocess.run([binary], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout
