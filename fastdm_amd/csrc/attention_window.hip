@@ -507,7 +507,12 @@ static int launch_merge(const WindowParams& p, int rb_rows, hipStream_t s) {
   return FDM_OK;
 }
 
-// ---- host side: which form, and into how many parts
+// ---- host side: what the kernel's 32-bit numbers hold (places, rows and items; addresses are 64-bit).  Within these limits the plan's 64-bit counts are exact.
+static bool window_fits(int64_t batch, int64_t sq, int64_t sk, int64_t kv_heads, int64_t group) {
+  return batch <= (1 << 24) && sq <= (1 << 29) && sk <= (1 << 29) && sq * group <= (1 << 30) && batch * kv_heads <= (1 << 28);
+}
+
+// ---- which form, and into how many parts
 //   0  up to 32 rows (single tokens and the like), 32-key tiles: blocks of one wave, no barrier to wait at, four (head_dim 64: eight) of them on a CU, each
 //      with its own share of the list.  Four waves on a 128-key tile instead: 128 sequences of 512 keys, 32/8 heads x 128: 42 -> 59 us; one sequence,
 //      window 4096: 11 -> 15 us.
@@ -567,6 +572,7 @@ extern "C" {
 
 int64_t fdm_attn_window_workspace_bytes(int64_t batch, int64_t sq, int64_t sk, int q_heads, int kv_heads, int head_dim, int64_t window, int64_t sinks) {
   if (batch <= 0 || sq <= 0 || sk <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128) || window < 1 || sinks < 0) return 0;
+  if (!window_fits(batch, sq, sk, kv_heads, q_heads / kv_heads)) return 0;
   const WindowPlan w = window_plan(batch, sq, sk, kv_heads, q_heads / kv_heads, head_dim, window < sk ? window : sk, sinks < sk ? sinks : sk);
   return w.parts > 1 ? w.units * w.parts * w.rb_rows * (head_dim + 2) * 4 : 0;
 }
@@ -586,9 +592,8 @@ int fdm_attn_window(void* o, const void* q, const void* k, const void* v, const 
   if ((at & 15) || (strides & 7) || strides < 0) return FDM_ERR_INVALID;
   if ((reinterpret_cast<uintptr_t>(q_lens) | reinterpret_cast<uintptr_t>(kv_lens)) & 3) return FDM_ERR_INVALID;
   const int64_t group = q_heads / kv_heads;
-  // places, rows and items are 32-bit numbers in the kernel (addresses are 64-bit)
   if (k_tok_stride > (1 << 22) || v_tok_stride > (1 << 22)) return FDM_ERR_UNSUPPORTED;      // (a tile's lane offsets are 32-bit)
-  if (sk > (1 << 29) || sq > (1 << 29) || sq * group > (1 << 30) || batch > (1 << 24)) return FDM_ERR_UNSUPPORTED;
+  if (!window_fits(batch, sq, sk, kv_heads, group)) return FDM_ERR_UNSUPPORTED;
   const int64_t win = window < sk ? window : (sk > 0 ? sk : 1), snk = sinks < sk ? sinks : sk;      // the same keys, and no overflow
   const WindowPlan w = window_plan(batch, sq, sk, kv_heads, group, head_dim, win, snk);
   const int64_t items = w.units * w.parts;

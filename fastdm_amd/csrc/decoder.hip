@@ -400,7 +400,7 @@ int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, c
   (void)hipGetLastError();  // drop any stale error of an earlier, unrelated runtime call: FDM_CHECK_LAUNCH must see only ours
   if (batch < 0 || seq < 0 || q_heads < 0 || k_heads < 0 || head_size <= 0 || rot_dim <= 0 || (rot_dim & 1) || rot_dim > head_size)
     return FDM_ERR_INVALID;
-  if (batch == 0 || seq == 0 || q_heads + k_heads == 0) return FDM_OK;
+  if (batch == 0 || seq == 0 || (q_heads == 0 && k_heads == 0)) return FDM_OK;
   if (!turns || (reinterpret_cast<uintptr_t>(turns) & 7) || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out))) return FDM_ERR_INVALID;
   if (positions && position_bytes != 4 && position_bytes != 8) return FDM_ERR_INVALID;
   if (positions && (reinterpret_cast<uintptr_t>(positions) & (position_bytes - 1))) return FDM_ERR_INVALID;

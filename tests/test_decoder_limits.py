@@ -5,6 +5,8 @@ import subprocess
 
 import pytest
 
+from fastdm_amd import _native as N
+
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fastdm_amd", "csrc")
 
 
@@ -43,3 +45,14 @@ int main() {
     subprocess.run([compiler, "-std=c++17", "-O1", "-I", CSRC, str(source), "-o", binary], check=True)
     done = subprocess.run([binary], capture_output=True, text=True)
     assert done.returncode == 0, done.stdout
+
+
+@pytest.mark.parametrize("batch,sq,sk,heads", [(1 << 32, 1 << 29, 1 << 29, 1 << 30), (1 << 40, 1 << 40, 1 << 29, 1), (1 << 24, 1 << 29, 1 << 29, 1 << 30),
+                                               (1 << 62, 1, 1 << 29, 4), (1 << 24, 1, 1 << 20, 32)])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_window_attention_refuses_counts_past_its_numbers(batch, sq, sk, heads, head_dim):
+    """Sizes whose products pass 64 bits (a count of 0 units was divided by) or 2^28 pairs: an error, and no workspace."""
+    lib = N.lib()
+    assert lib.fdm_attn_window_workspace_bytes(batch, sq, sk, heads, heads, head_dim, sk, 0) == 0
+    assert lib.fdm_attn_window(4096, 8192, 12288, 16384, None, None, batch, sq, sk, heads, heads, head_dim, 512, 64, 512, 64, 512, 64, 512, 64, 0.125, sk, 0,
+                               None, 0, None) == -2
