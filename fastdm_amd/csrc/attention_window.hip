@@ -233,8 +233,9 @@ __global__ void __launch_bounds__(64 * WR * WK, OCC) attn_window_kernel(const Wi
       for (int e = (n == 0 ? 1 : 0); e < 16; ++e) mx = __builtin_amdgcn_fmed3f(mx, s[n][e], __builtin_inff());
     const float mt = cross_half_max(mx) * p.scale_log2e;
     if (__any(mt > m_run + RESCALE)) {
-      const float m_new = fmaxf(m_run, mt);
-      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      // row by row: a row that shares the wave with one that moves stays where it is (alpha 1), so its bits do not go by its neighbours
+      const float m_new = mt > m_run + RESCALE ? mt : m_run;
+      const float alpha = mt > m_run + RESCALE ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
       m_run = m_new;
       l_run *= alpha;
 #pragma unroll

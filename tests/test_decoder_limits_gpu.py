@@ -71,3 +71,51 @@ def test_window_attention_of_more_blocks_than_a_launch_holds():
     # one key: the weight is 2^(s - s') with s' = s up to its last bit, bf16(weight) = 1; the division by the unrounded weight is off by 2^-22 of the value, a
     # bf16 number: it rounds back to it
     assert bool((got.view(copies, rows, H * D) == v.view(1, rows, H * D)).all())
+
+
+# ================================================================================================ rows by themselves
+FORMS = [(2, 9, 700, 6, 2, 64, 300, 3), (2, 1, 900, 8, 1, 128, 500, 2), (3, 90, 400, 8, 2, 64, 200, 5), (2, 100, 500, 6, 2, 128, 150, 70),
+         (8, 300, 420, 12, 12, 64, 200, 5), (3, 411, 411, 56, 8, 128, 128, 1), (1, 515, 3000, 16, 4, 128, 2500, 0)]      # each form, G = 1 and more
+
+
+@pytest.mark.parametrize("B,S,L,Hq,Hk,D,window,sinks", FORMS)
+@pytest.mark.parametrize("fill", [float("nan"), float("inf"), 1e30, -1e30, "large"])
+def test_window_attention_rows_past_the_queries_change_no_bit(B, S, L, Hq, Hk, D, window, sinks, fill):
+    """What a padded batch holds past q_lens: the queries in front of it, which share waves with it, keep every bit."""
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    if S == 1:
+        pytest.skip("one query: nothing behind it")
+    g = gen(S + L + D)
+    q, k, v = randn(g, B, S, Hq * D, scale=1.5), randn(g, B, L, Hk * D), randn(g, B, L, Hk * D)
+    lengths = [max(1, S - 3 - 7 * b) for b in range(B)]
+    q_lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    other = q.clone()
+    for b, n in enumerate(lengths):
+        q[b, n:] = 0
+        other[b, n:] = randn(g, S - n, Hq * D, scale=500.0) if fill == "large" else fill
+    want = attend(q, k, v, Hq, Hk, D, window, sinks=sinks, q_lens=q_lens)
+    assert torch.isfinite(want).all() and torch.equal(attend(other, k, v, Hq, Hk, D, window, sinks=sinks, q_lens=q_lens), want)
+
+
+@pytest.mark.parametrize("B,S,L,Hq,Hk,D,window,sinks", FORMS)
+def test_window_attention_rows_do_not_go_by_their_neighbours(B, S, L, Hq, Hk, D, window, sinks):
+    """Other queries of the same wave that meet far larger scores, and a key that only some rows see with an infinity in it: the other rows keep every bit."""
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    g = gen(S * L + D)
+    q, k, v = randn(g, B, S, Hq * D, scale=1.5), randn(g, B, L, Hk * D), randn(g, B, L, Hk * D)
+    want = attend(q, k, v, Hq, Hk, D, window, sinks=sinks)
+    loud = q.view(B, S, Hq, D).clone()
+    row = torch.arange(S, device="cuda")[:, None] * Hq + torch.arange(Hq, device="cuda")[None]
+    loud[:, row % 3 == 1] *= 60.0
+    got = attend(loud.view_as(q), k, v, Hq, Hk, D, window, sinks=sinks)
+    quiet = (row % 3 != 1)[None, :, :, None].expand(B, S, Hq, D)
+    assert torch.equal(got.view(B, S, Hq, D)[quiet], want.view(B, S, Hq, D)[quiet])
+    if S > 1:
+        j = L - S // 2 - 1
+        for bad in (float("inf"), -float("inf")):
+            k2 = k.clone()
+            k2[:, j, ::D] = bad                  # one element of every kv head's key
+            got = attend(q, k2, v, Hq, Hk, D, window, sinks=sinks)
+            place = torch.arange(L - S, L, device="cuda")
+            sees = (place >= j) & ((place < j + window) | (j < sinks))
+            assert not sees.all() and torch.equal(got[:, ~sees], want[:, ~sees])
