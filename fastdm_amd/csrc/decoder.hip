@@ -33,6 +33,10 @@ struct NormArgs {
   float eps;
 };
 
+// the IEEE 754-2019 maximum and minimum, which keep a NaN (v_maximum3_f32, v_minimum3_f32), where fmaxf and fminf drop it
+struct OpMaximum { __device__ __forceinline__ float operator()(float a, float b) const { return __builtin_elementwise_maximum(a, b); } };
+struct OpMinimum { __device__ __forceinline__ float operator()(float a, float b) const { return __builtin_elementwise_minimum(a, b); } };
+
 // MODE 0: bf16, 1: e4m3, 2: int8.  EDGE: the width is no multiple of 8 or a row is not 16-byte aligned; the last vector may be short.
 template <int THREADS, int NIT, int MODE, bool RES, bool EDGE>
 __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(const NormArgs p) {
@@ -87,18 +91,18 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(const NormArgs p)
         if (!EDGE || v * 8 + j < p.width) ss = __builtin_fmaf(a.v[j], a.v[j], ss);
         if constexpr (MODE != 0) {
           const float t = a.v[j] * g.v[j];
-          if constexpr (MODE == 1) hi = fmaxf(hi, fabsf(t));
+          if constexpr (MODE == 1) hi = __builtin_elementwise_maximum(hi, fabsf(t));
           else {
-            hi = fmaxf(hi, t);
-            lo = fminf(lo, t);
+            hi = __builtin_elementwise_maximum(hi, t);
+            lo = __builtin_elementwise_minimum(lo, t);
           }
         }
       }
     }
   }
   ss = wave_reduce(ss, OpSum());
-  if constexpr (MODE != 0) hi = wave_reduce(hi, OpMax());
-  if constexpr (MODE == 2) lo = wave_reduce(lo, OpMin());
+  if constexpr (MODE != 0) hi = wave_reduce(hi, OpMaximum());
+  if constexpr (MODE == 2) lo = wave_reduce(lo, OpMinimum());
   if constexpr (NW > 1) {
     if ((tid & 63) == 0) {
       red[0][tid >> 6] = ss;
@@ -112,19 +116,20 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_kernel(const NormArgs p)
     if constexpr (MODE != 0) {
       hi = red[1][0];
 #pragma unroll
-      for (int k = 1; k < NW; ++k) hi = fmaxf(hi, red[1][k]);
+      for (int k = 1; k < NW; ++k) hi = __builtin_elementwise_maximum(hi, red[1][k]);
     }
     if constexpr (MODE == 2) {
       lo = red[2][0];
 #pragma unroll
-      for (int k = 1; k < NW; ++k) lo = fminf(lo, red[2][k]);
+      for (int k = 1; k < NW; ++k) lo = __builtin_elementwise_minimum(lo, red[2][k]);
     }
   }
   const float rs = 1.0f / sqrtf(ss / (float)p.width + p.eps);
 
   // 8-bit forms: y / s as y * (1 / s).  A row of zeros gets the scale of max|y| = 1e-12 (the row quantisers' floor); int8 rows whose values
   // lie closer together than 1/16 of their size get the scale of that spread, so that z stays small (a step is then 2^-12 of the values).
-  // A NaN anywhere in the row makes ss, so the scale and the row's e4m3 bytes, NaN (comparisons with NaN leave it in place).
+  // A NaN in the row makes ss NaN, and with it rs; a NaN product (an infinity times a weight of 0, a NaN weight) makes the extremes NaN; an infinite
+  // product makes them inf * 0.  Each way the scale, and so the row's e4m3 bytes, are NaN (comparisons with NaN leave it in place).
   float inv = 1.f, zero = 0.f;
   if constexpr (MODE == 1) {
     float amax = hi * rs;

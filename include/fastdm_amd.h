@@ -447,8 +447,10 @@ int fdm_qk_norm_rope_inplace(void* qkv, const void* wq, const void* wk, const vo
  *   quant_mode 2: out_scale = (max y - min y) / 255, out_azp = -128 - rint(min y / out_scale), out_q = rint(y / out_scale) + out_azp (the spread
  *   counts as at least max|y| / 16 and 1e-12: a row of one value stays representable).
  * x, res, h_out: [rows, width] bf16 with their own row strides (elements); outputs compact.  h_out may be x or res (not other rows of theirs).  Any
- * width <= 65536 and any (element) alignment; multiples of 8 on 16-byte aligned rows take whole vectors.  A row with a NaN or an infinity gives NaNs
- * (its 8-bit rows: a NaN scale); a row whose sum of squares passes fp32's range gives zeros.  rows <= 2^31 - 1 (in several launches where one does not
+ * width <= 65536 and any (element) alignment; multiples of 8 on 16-byte aligned rows take whole vectors.  What is not finite: a NaN in h makes
+ * its row NaN; an infinity in h gives NaN at its place and zeros beside it; 8-bit rows with an infinity in h or a NaN in
+ * h * weight (an infinity at a weight of 0, a NaN weight) have a NaN scale and NaN e4m3 bytes (int8's bytes and zero point say nothing); products past
+ * fp32's range an infinite scale.  A row whose sum of squares passes fp32's range gives zeros.  rows <= 2^31 - 1 (in several launches where one does not
  * hold the threads; so the other two entries).                                                                                              */
 int fdm_add_rms_norm(void* out_bf16, void* out_q, float* out_scale, int32_t* out_azp, int quant_mode, const void* x, const void* res,
                      const void* weight, void* h_out, int64_t rows, int64_t width, int64_t x_row_stride, int64_t res_row_stride,

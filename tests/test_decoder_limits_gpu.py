@@ -119,3 +119,40 @@ def test_window_attention_rows_do_not_go_by_their_neighbours(B, S, L, Hq, Hk, D,
             place = torch.arange(L - S, L, device="cuda")
             sees = (place >= j) & ((place < j + window) | (j < sinks))
             assert not sees.all() and torch.equal(got[:, ~sees], want[:, ~sees])
+
+
+# ================================================================================================ rows that are not finite
+@pytest.mark.parametrize("width", [8, 500, 1003, 5120, 8192, 40000])
+@pytest.mark.parametrize("quant", [None, FP8, torch.int8])
+def test_add_rms_norm_of_what_is_not_finite_at_any_weight(width, quant):
+    """A NaN or an infinity at a channel whose weight is 0, and a NaN weight: NaN where the formula gives NaN, a NaN scale for such 8-bit rows; others as ever."""
+    from fastdm_amd.kernel.fused import add_rms_norm
+    g = gen(width)
+    nan, inf = float("nan"), float("inf")
+    x, residual = randn(g, 9, width), randn(g, 9, width)
+    weight = (1 + 0.3 * torch.randn(width, generator=g, device="cuda")).to(BF16)
+    at = width - 1 if width % 8 else width // 2 + 3
+    weight[at] = 0
+    finite = add_rms_norm(x, residual, weight, 1e-6, quant=quant)
+    for row, value in ((1, nan), (3, inf), (5, -inf)):
+        x[row, at] = value
+    residual[7, at], x[7, at] = inf, -inf                      # their sum is NaN
+    bad = torch.tensor([1, 3, 5, 7], device="cuda")
+    good = torch.tensor([0, 2, 4, 6, 8], device="cuda")
+    out, z, h = add_rms_norm(x, residual, weight, 1e-6, quant=quant)
+    assert torch.equal(h[good], finite[2][good])
+    if quant is None:
+        assert torch.equal(out[good], finite[0][good]) and torch.isnan(out[bad, at]).all() and torch.isnan(out[[1, 7]]).all()
+        beside = torch.arange(width, device="cuda") != at
+        assert (out[[3, 5]][:, beside] == 0).all()
+    else:
+        assert torch.isnan(z.scale[bad]).all() and torch.equal(z.scale[good], finite[1].scale[good])
+        assert torch.equal(z.q.view(torch.uint8)[good], finite[1].q.view(torch.uint8)[good])
+        if quant == FP8:
+            assert torch.isnan(z.q[bad].float()).all()
+    weight[at] = nan
+    out, z, _ = add_rms_norm(randn(g, 3, width), None, weight, 1e-6, quant=quant)
+    if quant is None:
+        assert torch.isnan(out[:, at]).all() and torch.isfinite(out[:, torch.arange(width, device="cuda") != at]).all()
+    else:
+        assert torch.isnan(z.scale).all()
