@@ -339,6 +339,23 @@ def row_stride(t, what):
     return stride
 
 
+def meets_itself(width, shape, strides):
+    """Whether two of the rows (dense, `width` elements) of an output with two outer axes of these sizes and strides share memory."""
+    (s, n), (t, m) = sorted(zip(strides, shape))              # t: the wider stride
+    if n <= 1:
+        return n == 1 and m > 1 and t < width
+    if s < width:
+        return m > 0
+    if m <= 1 or t >= (n - 1) * s + width:
+        return False
+    # i wide steps on, the nearest rows lie i t - j s and its complement to s away
+    for i in range(1, min(m - 1, ((n - 1) * s + width - 1) // t) + 1):
+        j, rest = divmod(i * t, s)
+        if j < n and rest < width or j + 1 < n and s - rest < width:
+            return True
+    return False
+
+
 def crosses(a, out, same=False):
     """Whether `out` [.., rows, width], being written, lies across `a`: rows (dense, at any strides) that share memory.  The very same rows are in place
     and do not count, unless `same`.  Rows of equal strides may lie between each other's (slices of one tensor); of different strides, any common

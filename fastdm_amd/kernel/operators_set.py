@@ -63,7 +63,7 @@ def _rotary_side(x, out, B, S, head_size, what):
     assert out.shape == shape and out.dtype == BF16, f"rotary_positions: {what}_out as {what}"
     o_bs, o_ts, o_es = out.stride()
     assert o_es == 1, f"rotary_positions: {what}_out's tokens must be dense"
-    assert (S <= 1 or o_ts >= width) and (B <= 1 or o_bs >= width), f"rotary_positions: {what}_out overlaps itself"
+    assert not N.meets_itself(width, (B, S), (o_bs, o_ts)), f"rotary_positions: {what}_out overlaps itself"
     return out, width // head_size, x_bs, x_ts, o_bs, o_ts
 
 

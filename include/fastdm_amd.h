@@ -457,7 +457,7 @@ int fdm_add_rms_norm(void* out_bf16, void* out_q, float* out_scale, int32_t* out
                      int64_t h_row_stride, float eps, fdm_stream_t stream);
 
 /* Rotary positions at given places (ABI 21): q [batch, seq, q_heads * head_size] and k [batch, seq, k_heads * head_size] bf16 with batch and token
- * strides in elements, to q_out / k_out (their own strides; q_out == q and k_out == k with equal strides: in place).  Pair i of a head's first
+ * strides in elements, to q_out / k_out (their own strides, no two tokens of an output in one place; q_out == q and k_out == k with equal strides: in place).  Pair i of a head's first
  * rot_dim elements -- (2i, 2i + 1), or (i, i + rot_dim / 2) where is_neox -- turns by 2 pi * place * turns[i] and is scaled by amplitude; the rest of
  * the head is copied.  turns: fp64 [rot_dim / 2], turns per position; the angle's fraction of a turn is taken in 64 bits, sine and cosine in fp32.
  * positions: int32 / int64 (position_bytes 4 / 8) at positions[b * pos_batch_stride + s * pos_tok_stride], or NULL for 0 .. seq - 1.

@@ -56,3 +56,29 @@ def test_window_attention_refuses_counts_past_its_numbers(batch, sq, sk, heads, 
     assert lib.fdm_attn_window_workspace_bytes(batch, sq, sk, heads, heads, head_dim, sk, 0) == 0
     assert lib.fdm_attn_window(4096, 8192, 12288, 16384, None, None, batch, sq, sk, heads, heads, head_dim, 512, 64, 512, 64, 512, 64, 512, 64, 0.125, sk, 0,
                                None, 0, None) == -2
+
+
+def test_outputs_that_overlap_themselves_against_every_row():
+    """All small sizes and strides of two axes, against the places themselves."""
+    for B in range(4):
+        for S in range(6):
+            for width in (1, 2, 3):
+                for bs in range(14):
+                    for ts in range(14):
+                        rows = [b * bs + s * ts for b in range(B) for s in range(S)]
+                        places = [r + i for r in rows for i in range(width)]
+                        assert N.meets_itself(width, (B, S), (bs, ts)) == (len(set(places)) < len(places)), (B, S, width, bs, ts)
+
+
+def test_rotary_positions_refuses_an_output_whose_tokens_share_places(monkeypatch):
+    """Strides that are each as wide as a token, but bring two tokens to one place."""
+    import torch
+    from fastdm_amd.kernel.operators_set import _rotary_side
+    x = torch.zeros(2, 6, 128, dtype=torch.bfloat16)
+    for strides in ((128, 128, 1), (256, 128, 1), (640, 128, 1), (128, 130, 1), (192, 300, 1)):
+        memory = torch.zeros(4096, dtype=torch.bfloat16)
+        with pytest.raises(AssertionError, match="overlaps itself"):
+            _rotary_side(x, torch.as_strided(memory, (2, 6, 128), strides), 2, 6, 64, "key")
+    for strides in ((768, 128, 1), (128, 256, 1), (1408, 256, 1), (800, 130, 1), (1000, 136, 1), (192, 384, 1)):      # disjoint, interleaved ones among them
+        out = torch.as_strided(torch.zeros(8192, dtype=torch.bfloat16), (2, 6, 128), strides)
+        assert _rotary_side(x, out, 2, 6, 64, "key")[0] is out
