@@ -7,6 +7,7 @@ library cannot be found (or built in-tree with hipcc) importing a kernel raises.
 import ctypes as C
 import os
 import subprocess
+import sys
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -292,8 +293,12 @@ def ptr(t):
 
 
 def gpu_of(what, *tensors):
-    """Index of the GPU that holds every one of `tensors` (None entries are skipped); none may be one that autograd expects a gradient through (the
-    operators have no backward).  The first one is always there."""
+    """Index of the GPU that holds every one of `tensors` (None entries are skipped); none may be one that autograd expects a gradient through, or
+    that carries a forward-mode tangent (the operators have no backward and no forward derivative).  The first one is always there."""
+    forward_ad = sys.modules.get("torch.autograd.forward_ad")
+    if forward_ad is not None and getattr(forward_ad, "_current_level", 0) >= 0:      # (-1 outside of any dual level)
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise RuntimeError(f"{what}: no forward-mode derivative -- call it with tensors that carry no tangent")
     index = tensors[0].get_device()
     for t in tensors:
         if t is None:

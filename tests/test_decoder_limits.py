@@ -82,3 +82,23 @@ def test_rotary_positions_refuses_an_output_whose_tokens_share_places(monkeypatc
     for strides in ((768, 128, 1), (128, 256, 1), (1408, 256, 1), (800, 130, 1), (1000, 136, 1), (192, 384, 1)):      # disjoint, interleaved ones among them
         out = torch.as_strided(torch.zeros(8192, dtype=torch.bfloat16), (2, 6, 128), strides)
         assert _rotary_side(x, out, 2, 6, 64, "key")[0] is out
+
+
+def test_tangents_are_refused_instead_of_lost():
+    """A forward-mode dual tensor requires no gradient, but its tangent would end here without a word."""
+    import torch
+    import torch.autograd.forward_ad as forward_ad
+    from fastdm_amd.kernel.fused import add_rms_norm
+    from fastdm_amd.kernel.operators_set import rotary_positions, window_scaled_dot_product_attention
+    from fastdm_amd.layer.embeddings import RotaryFrequencies
+    x, w, f = torch.zeros(2, 64, dtype=torch.bfloat16), torch.ones(64, dtype=torch.bfloat16), RotaryFrequencies(64)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: add_rms_norm(dual, None, w, 1e-6), lambda: add_rms_norm(x, dual, w, 1e-6), lambda: rotary_positions(x[None], dual[None], 64, f),
+                     lambda: window_scaled_dot_product_attention(x[None], x[None], dual[None], 1, 1, 64, 4)):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+            with pytest.raises(RuntimeError, match="tangent"), torch.no_grad():
+                call()
+        with pytest.raises(RuntimeError, match="GPU"):                  # no tangent: the ordinary checks
+            add_rms_norm(x, None, w, 1e-6)

@@ -156,3 +156,22 @@ def test_add_rms_norm_of_what_is_not_finite_at_any_weight(width, quant):
         assert torch.isnan(out[:, at]).all() and torch.isfinite(out[:, torch.arange(width, device="cuda") != at]).all()
     else:
         assert torch.isnan(z.scale).all()
+
+
+def test_tangents_are_refused_on_the_gpu():
+    import torch.autograd.forward_ad as forward_ad
+    from fastdm_amd.kernel.fused import add_rms_norm
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    x, w = randn(gen(5), 4, 64), randn(gen(6), 64)
+    want = add_rms_norm(x, None, w, 1e-6)[0]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="tangent"):
+            add_rms_norm(dual, None, w, 1e-6)
+        with pytest.raises(RuntimeError, match="tangent"):
+            attend(x[None], dual[None], x[None], 1, 1, 64, 4)
+        assert torch.equal(add_rms_norm(x, None, w, 1e-6)[0], want)
+    for transform in (lambda: torch.func.jvp(lambda t: add_rms_norm(t, None, w, 1e-6)[0], (x,), (x,)),
+                      lambda: torch.func.grad(lambda t: add_rms_norm(t, None, w, 1e-6)[0].float().sum())(x)):
+        with pytest.raises(RuntimeError):
+            transform()
