@@ -175,3 +175,39 @@ def test_tangents_are_refused_on_the_gpu():
                       lambda: torch.func.grad(lambda t: add_rms_norm(t, None, w, 1e-6)[0].float().sum())(x)):
         with pytest.raises(RuntimeError):
             transform()
+
+
+# ================================================================================================ scores of every size
+@pytest.mark.parametrize("B,S,L,Hq,Hk,D,window,sinks", FORMS)
+@pytest.mark.parametrize("shape", ["above", "below", "climbing", "falling", "one key above"])
+def test_window_attention_of_scores_with_a_large_common_part(B, S, L, Hq, Hk, D, window, sinks, shape):
+    """Scores of up to 2^20 that are exact in fp32: all of them on a grid of 1/8 (queries on 1/2, keys on 1/4), so every sum of products is a whole number
+    of eighths under 2^21, and what is common to a row's scores cancels in its softmax without loss.
+
+    Then a weight is off by: the scale's rounding and the exponent's, 2^-23 of an exponent of at most 40 (smaller weights do not count), 2^x itself
+    (2^-22), the sums over keys in fp32 (under 300 steps of 2^-24 for rows and products together): under 2^-15; the weight is rounded to bf16, and the
+    result once more (2^-8 each)."""
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    g = gen(S + L + Hq + D)
+    q = torch.randint(-4, 5, (B, S, Hq, D), generator=g, device="cuda").double() / 2
+    k = torch.randint(-8, 9, (B, L, Hk, D), generator=g, device="cuda").double() / 4
+    v = randn(g, B, L, Hk, D)
+    q[..., 0] = 128.0
+    key = torch.arange(L, device="cuda")
+    common = {"above": torch.full_like(key, 8192), "below": torch.full_like(key, -8192), "climbing": 512 * (16 * key // L), "falling": -512 * (16 * key // L),
+              "one key above": torch.where(key % 97 == 50, 16, 0)}[shape]
+    k[..., 0] = common.double()[None, :, None]
+    assert torch.equal(q.to(BF16).double(), q) and torch.equal(k.to(BF16).double(), k)
+    scale = 2.0 ** -4
+    got = attend(q.to(BF16).view(B, S, Hq * D), k.to(BF16).view(B, L, Hk * D), v.view(B, L, Hk * D), Hq, Hk, D, window, sinks=sinks, scale=scale).view(B, S, Hq, D).double()
+    place = torch.arange(L - S, L, device="cuda")[:, None]
+    hidden = ~((key <= place) & ((place - key < window) | (key < sinks)))
+    for b in range(B):
+        for head in range(Hq):
+            kk, vv = k[b, :, head // (Hq // Hk)], v[b, :, head // (Hq // Hk)].double()
+            p = torch.softmax((q[b, :, head] @ kk.t() * scale).masked_fill(hidden, float("-inf")), -1)
+            want, size = p @ vv, p @ vv.abs()
+            tol = want.abs() * 2.0 ** -8 + size * (2.0 ** -8 + 2.0 ** -15) * (1 + 2.0 ** -8)
+            assert (tol < 0.01 * size + 1e-30).all()                     # (says something)
+            worst = ((got[b, :, head] - want).abs() - tol).max().item()
+            assert worst <= 0, f"{shape}: sequence {b}, head {head}: beyond by {worst:.3g}"
