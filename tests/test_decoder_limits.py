@@ -102,3 +102,17 @@ def test_tangents_are_refused_instead_of_lost():
                 call()
         with pytest.raises(RuntimeError, match="GPU"):                  # no tangent: the ordinary checks
             add_rms_norm(x, None, w, 1e-6)
+
+
+def test_yarn_ramp_by_hand():
+    """16 elements, base 10^4, 4096 places, factor 4.  Pair x turns n times within them at x = 8 ln(4096 / (2 pi n)) / ln 10^4: n = 32 at 2.618, n = 1 at 5.628.
+    The ramp runs from pair 2 (whole) to pair 6 (slowed by 4): 0, 1/4, 1/2, 3/4, 1; theta_i = 10^(-i / 2) before it."""
+    from fastdm_amd.layer.embeddings import RotaryFrequencies
+    kept = [1, 1, 1, 13 / 16, 10 / 16, 7 / 16, 1 / 4, 1 / 4]
+    got = RotaryFrequencies(16, scaling="yarn", factor=4.0, original_length=4096)
+    assert got.theta == pytest.approx([10 ** (-i / 2) * part for i, part in enumerate(kept)], rel=1e-14)
+    assert got.amplitude == pytest.approx(1.138629436111989, rel=1e-15)                    # 1 + ln 4 / 10
+    # 64 places: n = 32 at -0.993, so the ramp starts at pair 0; n = 1 at 2.016: it ends at pair 3
+    kept = [1, 1 - 1 / 3 * 0.75, 1 - 2 / 3 * 0.75, 1 / 4, 1 / 4, 1 / 4, 1 / 4, 1 / 4]
+    got = RotaryFrequencies(16, scaling="yarn", factor=4.0, original_length=64, attention_factor=1.0)
+    assert got.theta == pytest.approx([10 ** (-i / 2) * part for i, part in enumerate(kept)], rel=1e-14) and got.amplitude == 1.0
