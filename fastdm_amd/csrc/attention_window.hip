@@ -1,7 +1,8 @@
 // Causal attention with a sliding window and sinks for gfx950 (bf16, head_dim 64 or 128): prompts, chunks behind a cache, single tokens.
 //
 //   visible   the query at place p of its sequence sees key j iff  j <= p  and  (p - j < window  or  j < sinks).  The queries of a sequence are its
-//             last q_len tokens: row t is at place kv_len - q_len + t.  Rows at or past q_len, and rows that see nothing, are zeros.
+//             last q_len tokens: row t is at place kv_len - q_len + t.  Rows at or past q_len, rows that see nothing,
+//             and rows whose scores are all -inf, are zeros.
 //   rows      the q heads that share a kv head are packed with the tokens: row r of (batch, kv head) is token r / G, head r % G, G = q_heads / kv_heads --
 //             one K / V tile in LDS serves all G heads, a 32-row wave spans 32 / G tokens (less of a tile lies behind the mask), and a single
 //             token's G rows are one wave's rows.

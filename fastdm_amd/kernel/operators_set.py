@@ -268,8 +268,8 @@ def window_scaled_dot_product_attention(query: torch.Tensor, key: torch.Tensor, 
     """Causal attention whose queries see the last `window` keys (their own among them) and the first `sinks`: query [B, Sq, Hq*D], key / value
     [B, Sk, Hkv*D] (a cache, or slices of one: batch and token strides of any multiples of 8, 16-byte aligned), [B, Sq, Hq*D] out.  The queries of a sequence are the last of its tokens:
     row t is at place kv_len - q_len + t and sees key j iff j <= place and (place - j < window or j < sinks).  q_lens / kv_lens: int32 [B] on the GPU
-    for padded batches and part-filled caches (default Sq / Sk; lengths outside 0 .. Sq / Sk count as the nearest).  Rows past q_len and rows that see
-    nothing are zeros; keys past kv_len and keys no row sees may hold anything.  Prompts, chunks behind a cache, and single tokens (Sq = 1)."""
+    for padded batches and part-filled caches (default Sq / Sk; lengths outside 0 .. Sq / Sk count as the nearest).  Rows past q_len, rows that see
+    nothing and rows whose scores are all -inf are zeros; keys past kv_len and keys no row sees may hold anything.  Prompts, chunks behind a cache, and single tokens (Sq = 1)."""
     name = "window_scaled_dot_product_attention"
     gpu = N.gpu_of(name, query, key, value, q_lens, kv_lens)
     assert query.dtype == BF16 and key.dtype == BF16 and value.dtype == BF16, "window_scaled_dot_product_attention: bf16 only"

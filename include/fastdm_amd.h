@@ -473,7 +473,7 @@ int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, c
  *   aligned tensors; k's and v's token strides <= 2^22); q_heads a multiple of kv_heads; head_dim 64 or 128.
  *   q_lens, kv_lens: int32 [batch] on the device, or NULL for sq / sk (values outside 0 .. sq / sk count as the nearest).  The queries of a sequence are
  *   the last q_len of its kv_len tokens: row t < q_len is at place kv_len - q_len + t and sees key j iff j <= place and (place - j < window or j < sinks).
- *   Rows at or past q_len, and rows that see nothing, are zeros.  Keys at or past kv_len are not read; what a row does not see does not reach it, NaNs
+ *   Rows at or past q_len, rows that see nothing, and rows whose scores are all -inf, are zeros.  Keys at or past kv_len are not read; what a row does not see does not reach it, NaNs
  *   and infinities included; where a row sees one in v, its result is not finite (NaN also for an infinity).
  *   softmax(q k^T * scale) v with fp32 statistics, scale > 0; window >= 1 (>= sk: plain causal), sinks >= 0; sk, sq <= 2^29, batch <= 2^24,
  *   batch * kv_heads <= 2^28 (FDM_ERR_UNSUPPORTED beyond; the workspace's size is 0 there).

@@ -211,3 +211,18 @@ def test_window_attention_of_scores_with_a_large_common_part(B, S, L, Hq, Hk, D,
             assert (tol < 0.01 * size + 1e-30).all()                     # (says something)
             worst = ((got[b, :, head] - want).abs() - tol).max().item()
             assert worst <= 0, f"{shape}: sequence {b}, head {head}: beyond by {worst:.3g}"
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_window_attention_of_rows_whose_scores_are_all_minus_infinity(D):
+    """They have no softmax: zeros, as where a row sees nothing; one finite score beside them, and the row is that key's value."""
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    g = gen(D)
+    S, H = 90, 2
+    q, k, v = randn(g, 1, S, H * D).abs() + 1, randn(g, 1, S, H * D), randn(g, 1, S, H * D)
+    k[:, 10:60] = float("-inf")
+    got = attend(q, k, v, H, H, D, 8)[0]
+    place = torch.arange(S, device="cuda")
+    none = (place >= 17) & (place < 60)
+    assert (got[none] == 0).all() and torch.isfinite(got).all()
+    assert torch.equal(got[16], v[0, 9]) and torch.equal(got[60], v[0, 60])
