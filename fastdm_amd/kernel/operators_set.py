@@ -72,8 +72,8 @@ def rotary_positions(query: torch.Tensor, key: Optional[torch.Tensor], head_size
                      key_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Rotary embedding at given places: query [B, S, Hq * head_size] and key [B, S, Hk * head_size] (or None) turned at positions[b, s]
     (int32 / int64, [S] or [B, S]; None: 0 .. S - 1) by `frequencies` (layer/embeddings.py RotaryFrequencies: part of the head, scalings for long
-    contexts).  Next to rotary_pos_embedding, which reads a bf16 cos | sin table of positions 0 .. S - 1: here the angle is taken in 64 bits at any
-    place and the result is rounded once.  is_neox: pairs (i, i + rotary_dim / 2) instead of (2i, 2i + 1).  Inputs may be slices of a fused
+    contexts).  Next to rotary_pos_embedding, which reads a bf16 cos | sin table of positions 0 .. S - 1: here the angle is taken in 64 bits (2^-22 of a
+    turn or better at places up to 2^31) and the result is rounded once.  is_neox: pairs (i, i + rotary_dim / 2) instead of (2i, 2i + 1).  Inputs may be slices of a fused
     projection (any batch and token strides); returns (query_out, key_out), new tensors unless given -- `query` / `key` themselves for in place,
     a cache's slice for a key that is stored there; an output that lies across an input otherwise is refused."""
     gpu = N.gpu_of("rotary_positions", query, key, positions, query_out, key_out, frequencies.turns)
@@ -269,7 +269,8 @@ def window_scaled_dot_product_attention(query: torch.Tensor, key: torch.Tensor, 
     [B, Sk, Hkv*D] (a cache, or slices of one: batch and token strides of any multiples of 8, 16-byte aligned), [B, Sq, Hq*D] out.  The queries of a sequence are the last of its tokens:
     row t is at place kv_len - q_len + t and sees key j iff j <= place and (place - j < window or j < sinks).  q_lens / kv_lens: int32 [B] on the GPU
     for padded batches and part-filled caches (default Sq / Sk; lengths outside 0 .. Sq / Sk count as the nearest).  Rows past q_len, rows that see
-    nothing and rows whose scores are all -inf are zeros; keys past kv_len and keys no row sees may hold anything.  Prompts, chunks behind a cache, and single tokens (Sq = 1)."""
+    nothing and rows whose scores are all -inf are zeros; keys past kv_len and keys no row sees may hold anything.  Scores (with scale)
+    may reach 2^28 in magnitude.  Prompts, chunks behind a cache, and single tokens (Sq = 1)."""
     name = "window_scaled_dot_product_attention"
     gpu = N.gpu_of(name, query, key, value, q_lens, kv_lens)
     assert query.dtype == BF16 and key.dtype == BF16 and value.dtype == BF16, "window_scaled_dot_product_attention: bf16 only"

@@ -475,7 +475,8 @@ int fdm_rope_positions(void* q_out, void* k_out, const void* q, const void* k, c
  *   the last q_len of its kv_len tokens: row t < q_len is at place kv_len - q_len + t and sees key j iff j <= place and (place - j < window or j < sinks).
  *   Rows at or past q_len, rows that see nothing, and rows whose scores are all -inf, are zeros.  Keys at or past kv_len are not read; what a row does not see does not reach it, NaNs
  *   and infinities included; where a row sees one in v, its result is not finite (NaN also for an infinity).
- *   softmax(q k^T * scale) v with fp32 statistics, scale > 0; window >= 1 (>= sk: plain causal), sinks >= 0; sk, sq <= 2^29, batch <= 2^24,
+ *   softmax(q k^T * scale) v with fp32 statistics, scale > 0, for scores up to 2^28 in magnitude (a score's distance to the running maximum is off by half a
+ *   step of the maximum: common to the row, but past 2^31 it leaves 2^x's range); window >= 1 (>= sk: plain causal), sinks >= 0; sk, sq <= 2^29, batch <= 2^24,
  *   batch * kv_heads <= 2^28 (FDM_ERR_UNSUPPORTED beyond; the workspace's size is 0 there).
  * workspace: 16-byte aligned, >= fdm_attn_window_workspace_bytes(...) of the same arguments (0: none), rewritten by every call.                */
 int64_t fdm_attn_window_workspace_bytes(int64_t batch, int64_t sq, int64_t sk, int q_heads, int kv_heads, int head_dim, int64_t window, int64_t sinks);

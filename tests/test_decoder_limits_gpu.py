@@ -226,3 +226,26 @@ def test_window_attention_of_rows_whose_scores_are_all_minus_infinity(D):
     none = (place >= 17) & (place < 60)
     assert (got[none] == 0).all() and torch.isfinite(got).all()
     assert torch.equal(got[16], v[0, 9]) and torch.equal(got[60], v[0, 60])
+
+
+@pytest.mark.parametrize("B,S,L,Hq,Hk,D,window,sinks", FORMS)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_window_attention_of_scores_up_to_the_largest(B, S, L, Hq, Hk, D, window, sinks, sign):
+    """Scores between 2^27 and 2^28, 2^20 and more apart in any 64 keys in a row: the largest one's key alone counts, and its value comes out.  Its weight is
+    2^r, r what the maximum's rounding leaves (at most 16 at 2^28 * log2 e): no bf16 number, so it is rounded once in the product (2^-8) and not in the sum that
+    the product is divided by; the result is rounded once more (2^-8), and the fp32 steps between are under 2^-20."""
+    from fastdm_amd.kernel.operators_set import window_scaled_dot_product_attention as attend
+    g = gen(D + L)
+    q = torch.zeros(B, S, Hq, D, device="cuda")
+    k = torch.zeros(B, L, Hk, D, device="cuda")
+    v = randn(g, B, L, Hk, D)
+    key = torch.arange(L, device="cuda")
+    steps = (key * 37) % 127
+    q[..., 0], k[..., 0] = 2.0 ** 14, sign * 2.0 ** 13 * (1 + steps / 128)[None, :, None]
+    assert torch.equal(k.to(BF16).float(), k)
+    got = attend(q.to(BF16).view(B, S, Hq * D), k.to(BF16).view(B, L, Hk * D), v.view(B, L, Hk * D), Hq, Hk, D, 64, scale=1.0).view(B, S, Hq, D)
+    place = torch.arange(L - S, L, device="cuda")[:, None]
+    seen = (key <= place) & (place - key < 64)
+    best = (sign * steps).expand(S, L).masked_fill(~seen, -1000).argmax(1)
+    want = v[:, best].repeat_interleave(Hq // Hk, 2).double()
+    assert ((got.double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -8 + 2.0 ** -15)).all()
