@@ -20,8 +20,10 @@
 //             rows see starts over: product with the finite values, and a second product of marks for the rows that see one that is not.
 //   bound     prompts: the matrix core and the softmax's VALU work behind it, which overlap across the two blocks of a CU only in part: 16384 tokens, 32/8
 //             heads x 128, window 4096: 945 - 990 us (by box) = 0.97 - 1.02 PFLOP/s of visible pairs, where a large bf16 product reaches 1.19; MFMA busy
-//             half of the cycles, LDS conflicts 0.  head_dim 64: VALU issue (32 exp2 of 4 issue slots each beside 16 MFMAs per tile).  Small grids: the
-//             chain of one block's tiles.  Single tokens: HBM, 16 sequences, window 4096: 54 us = 5.0 TB/s with the merge.
+//             half of the cycles, VALU 47 %, LDS conflicts 0.  head_dim 64 (4 ragged prompts of 958 - 1531 tokens, 24 heads, window 512: 32 us): no one unit (MFMA busy
+//             16 %, VALU 37 %, waiting 38 %); 960 blocks on 768 places leave a second round in which a quarter of the places work, every masked tile, half of
+//             them here, passes over V in LDS between its arrival and the barrier, and the softmax takes about twice the products' cycles (its exponentials
+//             alone as many).  Small grids: the chain of one block's tiles (about 1 us each for a single token).  Single tokens: HBM, 16 sequences, window 4096: 54 us = 5.0 TB/s with the merge.
 //   tried     fragments read a group ahead behind scheduling fences (+3 .. 15 %, spills), a three- or four-deep ring (+1 / +12 % at head_dim 64), the
 //             next tile's scores under this tile's softmax (spills at head_dim 128; +10 % at 64), s_setprio around either phase (+1 %), the row sums by
 //             v_dot2 (0), 128-key tiles with eight waves (+6 %), 32-key tiles (+7 %): none of them stayed.

@@ -25,9 +25,9 @@ struct Swz {
 
 // max over the two 32-lane halves of a wave (the two halves of a query row's keys), identical in both halves afterwards.
 // NOT `__builtin_amdgcn_permlane32_swap(x, x)` + fmaxf of the two results: hipcc 7.2 folds that to the first result alone (it takes the
-// swap of a value with itself for the identity), i.e. every lane got the LOWER half's maximum -- rounds 1-4 shipped that: harmless for the
-// bf16 kernels' results (a missed fix-up only lets P grow, bf16 has the exponent range) but it defeats the lazy row reference for half of
-// the keys, and with e4m3 P (fp8 P.V) a missed fix-up is a NaN.  Found with the spiked-key check of tools/micro/attn_bench (round 5).
+// swap of a value with itself for the identity), i.e. every lane gets the LOWER half's maximum: harmless for the bf16 kernels' results (a
+// missed fix-up only lets P grow, bf16 has the exponent range) but it defeats the lazy row reference for half of the keys, and with e4m3 P
+// (fp8 P.V) a missed fix-up is a NaN.  (The spiked-key check of tools/micro/attn_bench shows it.)
 // s_nop: VALU-written VGPR -> v_permlane32_swap needs a wait state that nothing pads inside asm.
 __device__ __forceinline__ float cross_half_max(float m) {
   float a = m, b = m;

@@ -55,7 +55,8 @@ for f in $UNITS; do
   extra=""
   [ "$f" = attention ] && extra="-fno-slp-vectorize -save-temps=obj"
   [ "$f" = gemm ] && extra="-save-temps=obj -Werror=inline-asm"     # (an asm clobber list naming a reserved register is an error)
-  # the decoder-side units: no packed-fp32 instructions (hipcc makes them of ordinary float code; some of their forms have given wrong results on these cards)
+  # the decoder-side units: no packed-fp32 instructions (hipcc makes them of ordinary float code; some of their forms have given wrong results on these cards).
+  # The flag also reaches the host pass, which warns that it does not know the feature: harmless
   [ "$f" = decoder ] || [ "$f" = attention_window ] && extra="-Xclang -target-feature -Xclang -packed-fp32-ops"
   # attention_window: MFMA results in vector registers also where one wave per SIMD could have accumulation registers too (a softmax reads every one of
   # them: one token, window 4096, 32/8 heads x 128: 11.0 -> 10.0 us)

@@ -13,11 +13,14 @@ typedef i32x2 i32x2_u __attribute__((aligned(1)));
 //   h = bf16(x + res)                 (the residual stream is kept in bf16; without res: h = x)
 //   y = h * w * rsqrt(mean(h^2) + eps)            in fp32, ONE rounding at the output:
 //   bf16(y)  |  e4m3(y / s), s = max|y| / 448  |  int8: rint(y / s) + z, s = (max y - min y) / 255, z = -128 - rint(min y / s)
-// One block per row, the row in registers: the block's one reduction carries the sum of squares and the extremes of h * w together (the
+// One block per row, the row in registers (from 32769 columns on six of the twelve forms spill 20 .. 172 bytes a thread): the block's one reduction carries the sum of squares and the extremes of h * w together (the
 // extremes of y are theirs times the row's rsqrt: a product with one positive factor keeps the order, roundings included).
-// Bound: HBM, 7 bytes per element (8 with a bf16 output).  16384 x 5120 to e4m3: 101 us = 5.8 TB/s (a copy of 300 MB: 5.4); 4099 x 3584 to bf16: 18 us; one
-// row of 4096: 2.4 us, the launch.  Threads per row (launch_norm's callers): 64 / 128 / 256 / 512 / 1024 threads take, 16384 rows to e4m3, for 512 columns
-// 11.8 / 14.5 / 21 / 37 / 75 us, for 4096 87 / 85 / 83 / 83 / 117 us, for 5120 - / 105 / 103 / 105 / 131 us; 8192 rows of 8192 - / 88.4 / 86.2 / 84.6 / 86.4 us.
+// Bound: HBM, 7 bytes per element (8 with a bf16 output).  16384 x 5120 to e4m3: 100 us = 5.8 TB/s (a copy of 300 MB: 5.4), to int8 the same; 4099 x 3584 to
+// bf16: 18 us; one row of 4096: 2.6 us, the launch; 1023 x 1536 to int8: 5.0 - 6 us, one round of blocks that wait for memory (67 % of their waves' cycles).
+// 2048 x 65536 to e4m3: 190 us = 4.9 TB/s, to int8 206 us; without a residual, where most of the spills are, 156 and 190 us for 3 bytes per element (bf16, 4 bytes: 108 us).
+// Threads per row (fdm_add_rms_norm): 64 / 128 / 256 / 512 / 1024 threads take, 16384 rows to e4m3, for 512 columns 11.8 / 14.5 / 21 / 37 / 75 us, for 4096
+// 87 / 85 / 83 / 83 / 117 us, for 5120 - / 105 / 103 / 105 / 131 us; 8192 rows of 8192 - / 88.4 / 86.2 / 84.6 / 86.4 us.  Up to 512 columns take 64 threads, the
+// others 256 and more.  There is no form of 128: 520 to 1024 columns pay for idle lanes (16384 rows of 520 / 768 / 1024: 22 / 23 / 24 us, 2.7 / 3.9 / 4.9 TB/s).
 struct NormArgs {
   bf16_t* out;
   uint8_t* q;
@@ -217,7 +220,8 @@ static int launch_norm(NormArgs a, int64_t rows, int mode, bool edge, hipStream_
 // A block takes a few tokens: their sines and cosines once into LDS (a 64-bit product and about 40 fp32 instructions each, shared by all heads), then
 // every head of q and k from there.
 // Bound: HBM, 4 bytes per element.  16384 tokens, 40 heads x 128: 64 us = 5.25 TB/s (a copy: 5.4); 3 x 1371 tokens, 48 heads x 64, half of each head
-// rotated: 10.1 us (13.6 with one item at a time and divisions by the items per token and head); 32 single tokens: 4.2 us.
+// rotated: 10.1 us (13.6 with one item at a time and divisions by the items per token and head); 32 single tokens: 4.8 us, two memory latencies in a
+// row (the places, then q and k behind the sines and cosines).
 struct RopeAtArgs {
   const bf16_t* q;
   const bf16_t* k;

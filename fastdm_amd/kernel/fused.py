@@ -96,7 +96,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
     where an addition, rms_norm and quantize_rows take three, and ONE rounding of y (it is not rounded to bf16 on its way to 8 bits).
     x, residual: [rows, width] bf16, rows may be column slices of wider matrices.  Returns (bf16 y | None, Quantized | None, h | None) like ln_modulate.
     residual_out: where h goes (may be `residual` or `x` itself: in place; not across either of them).  residual=None: the norm of x alone, h is None.
-    e4m3: scale = max|y| / 448; int8: asymmetric (scale, azp), as the row quantisers."""
+    e4m3: scale = max|y| / 448; int8: asymmetric (scale, azp) as the row quantisers, but the spread counts as at least max|y| / 16 (they have no such floor).
+    Rows that are not finite have a NaN scale, products h * weight past fp32's range an infinite one."""
     gpu = N.gpu_of("add_rms_norm", x, residual, weight, residual_out)
     assert x.ndim == 2 and x.dtype == BF16 and weight.dtype == BF16, "add_rms_norm: x [rows, width] and weight in bf16"
     rows, width = shape = x.shape
